@@ -21,7 +21,8 @@ MPC_ORDER_ADD_THEN_ROUND = 1
 MPC_BITS_LOG2 = 0
 MPC_BITS_LN = 1
 MPC_CONV, MPC_DECONV = 0, 1
-MPC_ACT_NONE, MPC_ACT_GDN, MPC_ACT_IGDN, MPC_ACT_RELU, MPC_ACT_EXP = 0, 1, 2, 3, 4
+MPC_ACT_NONE, MPC_ACT_GDN, MPC_ACT_IGDN, MPC_ACT_RELU, MPC_ACT_EXP, MPC_ACT_GELU, MPC_ACT_SILU = 0, 1, 2, 3, 4, 5, 6
+MPC_TYPE_F32, MPC_TYPE_F16, MPC_TYPE_BF16, MPC_TYPE_E4M3 = 0, 1, 2, 3
 MPC_IN_ABS, MPC_OUT_ROUND, MPC_OUT_CLAMP01, MPC_OUT_NCHW, MPC_F16, MPC_F16X3, MPC_WIDE_BLOCK, MPC_OUT_SPLIT = 1, 2, 4, 8, 16, 32, 64, 128
 
 
@@ -32,6 +33,11 @@ class MpcError(RuntimeError):
 class ConvDesc(ctypes.Structure):
     _fields_ = [(n, c_int32) for n in ("kind", "cin", "cout", "ksize", "stride", "pad", "out_pad", "act", "flags")] + \
                [("in_bound", c_float)]
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [(n, c_int32) for n in ("in_type", "out_type", "act")] + \
+               [(n, c_int64) for n in ("M", "N", "K", "x_stride", "w_stride", "residual_stride", "out_stride")]
 
 
 # name -> (restype, argtypes); every symbol declared in include/mpc.h
@@ -92,6 +98,16 @@ SIGNATURES = {
     "mpc_f16_to_f32": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "mpc_laplace_bits": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "mpc_prob_bits": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "mpc_rms_norm": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_float, c_int, c_void_p,
+                             c_void_p, c_int, c_void_p]),
+    "mpc_linear_workspace_bytes": (c_size_t, [POINTER(LinearDesc)]),
+    "mpc_linear_forward": (c_int, [c_void_p, POINTER(LinearDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_size_t, c_void_p]),
+    "mpc_prior_balance_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "mpc_prior_balance": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int64, c_int64, c_float, c_int, c_void_p, c_void_p,
+                                  c_size_t, c_void_p, c_void_p, c_void_p]),
+    "mpc_prior_balance_grad": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_int64, c_int64, c_float, c_int, c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64]),
     "mpc_laplace_cdf_rows": (c_int, [c_void_p, c_void_p, c_int64, c_float, c_int, c_int, c_void_p]),
 }
 

@@ -502,6 +502,7 @@ int mpc_conv_create(mpc_ctx *ctx, const mpc_conv_desc *desc, const float *weight
     MPC_REQUIRE(ctx, d.stride == 1 || d.stride == 2, "conv_create: stride must be 1 or 2");
     MPC_REQUIRE(ctx, d.kind == MPC_CONV ? d.out_pad == 0 : d.out_pad == d.stride - 1, "conv_create: out_pad must be stride-1 for deconv, 0 for conv");
     MPC_REQUIRE(ctx, !gdn || (beta && gamma), "conv_create: GDN needs beta and gamma");
+    MPC_REQUIRE(ctx, d.act >= MPC_ACT_NONE && d.act <= MPC_ACT_EXP, "conv_create: activation %d is not one of a convolution's", d.act);
     const bool cin4 = d.cin <= 4;
     const bool stacked = d.kind == MPC_DECONV && d.stride == 2 && d.cout * 4 <= 32;
     const bool f16 = (d.flags & MPC_F16) != 0;

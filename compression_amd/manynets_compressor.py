@@ -244,7 +244,7 @@ class Balle2017ManyPriors_ImageCompressor(abstract_model.AbstractHyperpriorImage
             "host_bits": {"feature": bits_host, "sidestring": float(side_bits)},
         }
 
-    def _forward_train(self, input_image, quant_noise=None, **kwargs):
+    def _forward_train(self, input_image, quant_noise=None, prior_balance=False, **kwargs):
         """Training-mode forward (manynets_compressor.py:514-530, 547-607, 621-625): the rate is estimated on
         y + U(-0.5, 0.5) by the K priors' networks themselves (the latent is not an integer, so no table applies), the
         decoder sees round(y) (passthrough_ae) or the noisy latent, priors unused for more than 50 calls are forced onto
@@ -252,7 +252,12 @@ class Balle2017ManyPriors_ImageCompressor(abstract_model.AbstractHyperpriorImage
 
         `quant_noise` ([B, M, h, w], the reference's layout) replaces the noise this method would draw with
         torch's generator on the device.  The returned tensors are values only: libmpc has no backward pass, so
-        nothing here carries an autograd graph."""
+        nothing here carries an autograd graph.
+
+        `prior_balance=True` (not in the reference, whose remedy for idle priors is forcing them) adds how evenly the
+        competition uses its priors: "prior_balance" (ops.prior_balance of the priors' bits, a location's weight of a
+        prior being 2^-bits; 1 = all alike, K = one takes everything), "prior_counts" (int32 [K], locations each prior
+        won, before forcing) and "prior_balance_grad" (its gradient in those bits, fp32 [n_loc, K])."""
         x = input_image.contiguous()
         B, _, H, W = x.shape
         npix = B * H * W
@@ -290,7 +295,7 @@ class Balle2017ManyPriors_ImageCompressor(abstract_model.AbstractHyperpriorImage
         bpp_feature = torch.tensor(bits / npix, dtype=torch.float32, device=x.device)
         # as in the reference, whose feature_batched_shape[0] is the batch size in this layout (:555, :621-625)
         bpp_sidestring = torch.tensor((B * math.log2(K)) / npix)
-        return {
+        out = {
             "reconstructed_image": xhat,
             "visual_loss": visual_loss,
             "bpp_feature": bpp_feature,
@@ -299,6 +304,11 @@ class Balle2017ManyPriors_ImageCompressor(abstract_model.AbstractHyperpriorImage
             "used_dists": used.tolist(),
             "num_forced_dists": num_forced,
         }
+        if prior_balance:
+            costs = total.t()                            # [n_loc, K], prior by prior in memory
+            out["prior_balance"], out["prior_counts"], n_rows = ops.prior_balance(costs, scale=-math.log(2.0))
+            out["prior_balance_grad"] = ops.prior_balance_grad(costs, out["prior_counts"], n_rows, scale=-math.log(2.0))
+        return out
 
     def _encode_symbols(self, sym, idx, n_images, est_bytes_per_image, verify=False):
         """sym int16 [n_images*n_loc, M], idx int32 [n_images*n_loc] -> (list of MRS1 byte strings, geometry)."""

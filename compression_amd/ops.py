@@ -277,6 +277,176 @@ def prior_bits_network(params: Sequence[torch.Tensor], y: torch.Tensor, K: int, 
     return idx, minbits, total, ye
 
 
+# ---- row operators: norm, matrix product, balance of the competition ------------------------------------------------
+_ROW_TYPES = {torch.float32: _lib.MPC_TYPE_F32, torch.float16: _lib.MPC_TYPE_F16, torch.bfloat16: _lib.MPC_TYPE_BF16}
+_OPERAND_TYPES = {torch.float16: _lib.MPC_TYPE_F16, torch.bfloat16: _lib.MPC_TYPE_BF16, torch.float8_e4m3fn: _lib.MPC_TYPE_E4M3}
+_LINEAR_ACTS = (_lib.MPC_ACT_NONE, _lib.MPC_ACT_RELU, _lib.MPC_ACT_GELU, _lib.MPC_ACT_SILU)
+
+
+def _rows(t: torch.Tensor, name: str) -> Tuple[int, int]:
+    """(rows, elements from one row to the next) of a [..., C] tensor whose rows are evenly spaced, C values of a row
+    consecutive.  A view that keeps neither is refused rather than copied."""
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise MpcError(f"{name} must have rows of at least one value, got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t.numel() // t.shape[-1], t.shape[-1]
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise MpcError(f"{name}: the values of a row must be consecutive (strides {t.stride()})")
+    rows, step = 1, 0
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if rows == 1:
+            step = stride
+        elif stride != step * rows:
+            raise MpcError(f"{name}: rows must be evenly spaced (shape {tuple(t.shape)}, strides {t.stride()})")
+        rows *= size
+    return rows, step
+
+
+def _same_gpu(x: torch.Tensor, **others):
+    if not x.is_cuda:
+        raise MpcError(f"tensors must live on the GPU (got {x.device}); compression_amd has no CPU path")
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise MpcError(f"{name} is on {t.device}, the input on {x.device}")
+
+
+def _vector(t: Optional[torch.Tensor], n: int, name: str):
+    if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
+        raise MpcError(f"{name} must be {n} contiguous float32 values, got {t.dtype} {tuple(t.shape)}")
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+             quantize: bool = False):
+    """Root-mean-square norm over the last axis: h = x + residual, v = h / sqrt(mean(h^2) + eps) * weight.
+
+    x, residual: [..., C] fp32, fp16 or bf16, rows evenly spaced (a slice of wider rows is fine), residual of x's shape and
+    type; weight fp32 [C] or None.  -> v in x's type, or with quantize (q, scale): e4m3 values [..., C] and fp32 [...],
+    v ~ q * scale, what `linear` takes as x and x_scale.  With a residual h (x's type, rounded once; the norm is taken of
+    the unrounded sum) is returned behind them: (v, h) or (q, scale, h).  Rows of zeros have scale 1.  Values only, like the
+    rest of the library: no autograd graph."""
+    _same_gpu(x, weight=weight, residual=residual)
+    if x.dtype not in _ROW_TYPES:
+        raise MpcError(f"rms_norm: x must be float32, float16 or bfloat16 (got {x.dtype})")
+    rows, xs = _rows(x, "x")
+    C = x.shape[-1]
+    _vector(weight, C, "weight")
+    rs = 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise MpcError(f"rms_norm: residual {residual.dtype} {tuple(residual.shape)} does not match x {x.dtype} {tuple(x.shape)}")
+        _, rs = _rows(residual, "residual")
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if quantize else x.dtype, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quantize else None
+    t = _ROW_TYPES[x.dtype]
+    if rows:
+        with _timed("rms_norm", bytes=float(x.numel()) * (x.element_size() * (1 if residual is None else 3) + y.element_size())):
+            context_for(x.device).call("mpc_rms_norm", ptr(x), xs, ptr(residual), rs, ptr(weight), rows, C, float(eps), t, ptr(h), ptr(y),
+                                       _lib.MPC_TYPE_E4M3 if quantize else t, ptr(scale))
+    out = ((y, scale) if quantize else (y,)) + (() if h is None else (h,))
+    return out if len(out) > 1 else y
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: int = _lib.MPC_ACT_NONE,
+           residual: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None,
+           weight_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x @ weight.T * x_scale * weight_scale + bias) + residual, in one pass.
+
+    x [..., K] and weight [N, K], both fp16, both bf16 or both e4m3 (torch.float8_e4m3fn), rows evenly spaced; bias fp32
+    [N]; act MPC_ACT_NONE, _RELU, _GELU (the erf form) or _SILU; residual [..., N] in the output's type.  e4m3 operands
+    bring their scales, fp32: x_scale [...] (one per row) and weight_scale [N]; 16-bit ones have none.  out_dtype: fp32,
+    fp16 or bf16; default the residual's type, else x's, and fp16 for e4m3 operands.  Sums and epilogue in fp32, one
+    rounding at the end.  Values only: no autograd graph."""
+    _same_gpu(x, weight=weight, bias=bias, residual=residual, x_scale=x_scale, weight_scale=weight_scale)
+    if x.dtype not in _OPERAND_TYPES or weight.dtype != x.dtype:
+        raise MpcError(f"linear: x and weight must both be float16, bfloat16 or float8_e4m3fn (got {x.dtype}, {weight.dtype})")
+    if act not in _LINEAR_ACTS:
+        raise MpcError(f"linear: activation {act} is not one of {_LINEAR_ACTS}")
+    if weight.dim() != 2 or weight.shape[0] == 0 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
+        raise MpcError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
+    M, xs = _rows(x, "x")
+    N, ws = _rows(weight, "weight")
+    eight = x.dtype == torch.float8_e4m3fn
+    if eight != (x_scale is not None) or eight != (weight_scale is not None):
+        raise MpcError("linear: e4m3 operands need x_scale and weight_scale, 16-bit operands take none")
+    _vector(bias, N, "bias")
+    _vector(x_scale, M, "x_scale")
+    _vector(weight_scale, N, "weight_scale")
+    odt = out_dtype if out_dtype is not None else residual.dtype if residual is not None else torch.float16 if eight else x.dtype
+    if odt not in _ROW_TYPES:
+        raise MpcError(f"linear: output type {odt} is not float32, float16 or bfloat16")
+    shape, rs = x.shape[:-1] + (N,), 0
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != odt:
+            raise MpcError(f"linear: residual {residual.dtype} {tuple(residual.shape)} does not match the output {odt} {tuple(shape)}")
+        _, rs = _rows(residual, "residual")
+    out = torch.empty(shape, dtype=odt, device=x.device)
+    if M == 0:
+        return out
+    K = x.shape[-1]
+    desc = _lib.LinearDesc(_OPERAND_TYPES[x.dtype], _ROW_TYPES[odt], act, M, N, K, xs, ws, rs, N)
+    ctx = context_for(x.device)
+    ws_bytes = ctx.lib.mpc_linear_workspace_bytes(ctypes.byref(desc))
+    work = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    with _timed("linear", flops=2.0 * M * N * K):
+        ctx.call("mpc_linear_forward", ctypes.byref(desc), ptr(x), ptr(x_scale), ptr(weight), ptr(weight_scale), ptr(bias), ptr(residual),
+                 ptr(work), ws_bytes, ptr(out))
+    return out
+
+
+def _balance_args(scores, scale, top_k, mask):
+    _same_gpu(scores, mask=mask)
+    if scores.dim() != 2 or scores.dtype not in _ROW_TYPES:
+        raise MpcError(f"prior_balance: scores must be [rows, experts] float32, float16 or bfloat16 (got {scores.dtype} {tuple(scores.shape)})")
+    T, E = scores.shape
+    if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (T,) or not mask.is_contiguous()):
+        raise MpcError(f"prior_balance: mask must be {T} contiguous bool values, got {mask.dtype} {tuple(mask.shape)}")
+    return (ptr(scores), _ROW_TYPES[scores.dtype], T, E, scores.stride(0), scores.stride(1), float(scale), int(top_k), ptr(mask))
+
+
+def prior_balance(scores: torch.Tensor, scale: float = 1.0, top_k: int = 1, mask: Optional[torch.Tensor] = None):
+    """How evenly the experts of a choice are used: -> (loss fp32 scalar, counts int32 [E], n_rows int32 [1]).
+
+    scores [rows, E] fp32, fp16 or bf16 in any layout (the competition's totals [K, n_loc] as `totals.t()` with a negative
+    scale: costs in bits weigh -ln 2); p = softmax(scale * scores).  Every row that counts (mask true, something above
+    -infinity) chooses its top_k best, ties to the lowest index.  loss = E * sum_e f_e P_e with f the share of the choices and
+    P the mean of p: 1 for even use, up to E where one expert takes all; 0 without rows.  counts are the choices per
+    expert.  Everything stays on the device; the order of the sums is fixed."""
+    args = _balance_args(scores, scale, top_k, mask)
+    T, E = scores.shape
+    dev = scores.device
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    n_rows = torch.empty(1, dtype=torch.int32, device=dev)
+    ctx = context_for(dev)
+    ws_bytes = ctx.lib.mpc_prior_balance_workspace_bytes(T, E)
+    work = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _timed("prior_balance", bytes=float(scores.numel()) * scores.element_size()):
+        ctx.call("mpc_prior_balance", *args, ptr(work), ws_bytes, ptr(loss), ptr(counts), ptr(n_rows))
+    return loss, counts, n_rows
+
+
+def prior_balance_grad(scores: torch.Tensor, counts: torch.Tensor, n_rows: torch.Tensor, grad_out: Optional[torch.Tensor] = None,
+                       scale: float = 1.0, top_k: int = 1, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of prior_balance's loss in the scores, in their type and layout, times grad_out (fp32, one value on the
+    device; None: 1).  counts and n_rows are what prior_balance returned for the same scores, scale, top_k and mask.  The
+    choices count as constants, as usual for this loss; rows that do not count get zeros."""
+    _same_gpu(scores, counts=counts, n_rows=n_rows, grad_out=grad_out)
+    args = _balance_args(scores, scale, top_k, mask)
+    E = scores.shape[1]
+    for t, n, name in ((counts, E, "counts"), (n_rows, 1, "n_rows")):
+        if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+            raise MpcError(f"prior_balance_grad: {name} must be {n} contiguous int32 values, got {t.dtype} {tuple(t.shape)}")
+    _vector(grad_out, 1, "grad_out")
+    grad = torch.empty_like(scores)
+    with _timed("prior_balance_grad", bytes=2.0 * scores.numel() * scores.element_size()):
+        context_for(scores.device).call("mpc_prior_balance_grad", *args, ptr(counts), ptr(n_rows), ptr(grad_out), ptr(grad), grad.stride(0),
+                                        grad.stride(1))
+    return grad
+
+
 def gather_cdf(table: torch.Tensor, idx: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """table int16 [K,M,L], idx int32 [n_loc] -> int16 [n_loc, M, L] (written into `out` when given)."""
     _dev(table, torch.int16, "table")

@@ -244,7 +244,9 @@ enum {
     MPC_ACT_GDN = 1,  /* y / sqrt(beta + gamma y^2)          GDN.py:83-91 */
     MPC_ACT_IGDN = 2, /* y * sqrt(beta + gamma y^2) */
     MPC_ACT_RELU = 3,
-    MPC_ACT_EXP = 4   /* SynthesisTFCodeExp_prior_net, Balle2018PT_compressor.py:248-251 */
+    MPC_ACT_EXP = 4,  /* SynthesisTFCodeExp_prior_net, Balle2018PT_compressor.py:248-251 */
+    MPC_ACT_GELU = 5, /* y/2 (1 + erf(y / sqrt 2)); mpc_linear_forward only */
+    MPC_ACT_SILU = 6  /* y / (1 + exp(-y)); mpc_linear_forward only */
 };
 enum {
     MPC_F16 = 16,          /* layer flag: fp16 operands / fp32 accumulate; activations in and out are fp16 NHWC
@@ -335,6 +337,63 @@ int mpc_prob_bits(mpc_ctx *ctx, const float *cdf_hi, const float *cdf_lo, int64_
  * order): out [n][L].  abstract_model.py:404-416. */
 int mpc_laplace_cdf_rows(mpc_ctx *ctx, const float *sigma, int64_t n, float first_target, int L,
                          int precision, int16_t *out);
+
+/* ---- row operators: [rows][channels] data outside the convolutions ----------------------------------------- */
+/* Types of their operands.  e4m3: 8 bits, 4 of exponent, 3 of mantissa, largest finite value 448, no infinities. */
+enum { MPC_TYPE_F32 = 0, MPC_TYPE_F16 = 1, MPC_TYPE_BF16 = 2, MPC_TYPE_E4M3 = 3 };
+
+/* Root-mean-square norm of rows, with the residual's addition on the way in and, if wanted, an 8-bit output:
+ *   h = x + residual,   v[c] = h[c] / sqrt(mean_c h^2 + eps) * weight[c].
+ * x, residual (may be NULL): `type` (F32, F16 or BF16), row i at element i * x_stride / i * residual_stride, the
+ * channels of a row consecutive.  weight (fp32 [channels], may be NULL: ones).  h (may be NULL): h rounded to `type`
+ * (the norm is taken of the unrounded sum), y: v, both dense [rows][channels].  y_type == type: v rounded once, scale
+ * must be NULL.  y_type == MPC_TYPE_E4M3: scale[i] = max_c |v| / 448, at least 2^-126, 1 for a row of zeros, and
+ * y = e4m3(v / scale[i]), nearest, ties to even.  A NaN anywhere in a row makes all of that row's y (and scale) NaN, an
+ * infinity makes its scale NaN.  Sums are in fp32: rows whose squares add up beyond 3e38 give zeros.
+ * Outputs overlap no input and no other output.  rows may be 0. */
+int mpc_rms_norm(mpc_ctx *ctx, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                 const float *weight, int64_t rows, int64_t channels, float eps, int type, void *h, void *y, int y_type,
+                 float *scale);
+
+/* Matrix product with its epilogue fused:
+ *   out[m][n] = act(x_scale[m] * w_scale[n] * sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n].
+ * x [M][K] and w [N][K] of in_type (F16, BF16 or E4M3), residual (may be NULL) and out [M][N] of out_type (F32, F16 or
+ * BF16); rows at multiples of the strides (in elements), values of a row consecutive.  bias (may be NULL) fp32 [N].
+ * x_scale fp32 [M] and w_scale fp32 [N]: with E4M3 operands, both; with 16-bit ones, NULL.  act: MPC_ACT_NONE, _RELU,
+ * _GELU or _SILU.  Sums and the epilogue are in fp32, out is rounded once.  out may be the residual itself (same
+ * address and stride); otherwise it overlaps no input.  M may be 0.  A work split over K goes through `workspace`
+ * (mpc_linear_workspace_bytes of the same description, 16-byte aligned; may be NULL where that is 0). */
+typedef struct {
+    int32_t in_type, out_type, act;
+    int64_t M, N, K;
+    int64_t x_stride, w_stride, residual_stride, out_stride;
+} mpc_linear_desc;
+size_t mpc_linear_workspace_bytes(const mpc_linear_desc *desc);
+int mpc_linear_forward(mpc_ctx *ctx, const mpc_linear_desc *desc, const void *x, const float *x_scale, const void *w,
+                       const float *w_scale, const float *bias, const void *residual, void *workspace,
+                       size_t workspace_bytes, void *out);
+
+/* How evenly the experts (the priors of a competition) are used, as a loss, with its gradient.  scores [rows][experts] of
+ * `type` (F32, F16, BF16) at element row * row_stride + expert * expert_stride (either layout of the competition's
+ * totals); z = scale * scores (scale finite, not 0; negative for costs), p = softmax(z) of a row.  A row counts if
+ * mask[row] != 0 (mask uint8, may be NULL) and it holds a z above -infinity (or a NaN).  It chooses its top_k largest z
+ * above -infinity, among equal ones those of the lowest index; a NaN is never chosen.  With R the rows that count,
+ *   counts[e] = rows that chose e,  f = counts / (top_k R),  P[e] = mean over those rows of p,
+ *   loss = experts * sum_e f[e] P[e]   (1 if every expert is used alike; 0 for R = 0).
+ * The gradient takes f as a constant:
+ *   grad[row][j] = grad_out * scale * experts / R * p[j] (f[j] - sum_e f[e] p[e]),  0 in rows that do not count.
+ * counts int32 [experts], n_rows int32 [1] (R), loss fp32 [1], all on the device; grad_out fp32 [1] on the device (NULL:
+ * 1).  rows * top_k < 2^31, experts <= 1024, 1 <= top_k <= experts; rows may be 0.  The order of every sum is fixed: the
+ * same call gives the same bits.  Replaces nothing of the reference: its remedy for idle priors is forcing them onto
+ * locations (manynets_compressor.py:583-607). */
+size_t mpc_prior_balance_workspace_bytes(int64_t rows, int experts);
+int mpc_prior_balance(mpc_ctx *ctx, const void *scores, int type, int64_t rows, int experts, int64_t row_stride,
+                      int64_t expert_stride, float scale, int top_k, const uint8_t *mask, void *workspace,
+                      size_t workspace_bytes, float *loss, int32_t *counts, int32_t *n_rows);
+int mpc_prior_balance_grad(mpc_ctx *ctx, const void *scores, int type, int64_t rows, int experts, int64_t row_stride,
+                           int64_t expert_stride, float scale, int top_k, const uint8_t *mask, const int32_t *counts,
+                           const int32_t *n_rows, const float *grad_out, void *grad, int64_t grad_row_stride,
+                           int64_t grad_expert_stride);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,579 @@
+"""Row operators (norm, matrix product, balance of the competition) against their definitions in 64 bits.
+
+Tolerances count roundings.  u(t) = finfo(t).eps / 2 is the largest relative error of one rounding to t, and half of the
+smallest subnormal its largest absolute one.  Sums of n terms in fp32 are off by at most n 2^-24 sum |terms| in any order
+(2^-23 where an instruction may truncate)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+torch.set_grad_enabled(False)
+
+F32, F16, BF16, E4M3 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn
+DEV = "cuda:0"
+TINY = {F32: 2.0 ** -150, F16: 2.0 ** -25, BF16: 2.0 ** -134}          # half of the smallest subnormal
+
+
+def u(t):
+    return torch.finfo(t).eps / 2
+
+
+def rnd(seed, *shape, scale=1.0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale
+
+
+def within(got, want, tol, what=""):
+    got, want, tol = got.double().to(want.device), want.double(), tol.double().to(want.device)
+    off = (got - want).abs()
+    bad = ~(off <= tol) & ~(torch.isnan(got) & torch.isnan(want)) & ~(got == want)
+    assert not bool(bad.any()), (what, int(bad.sum()), float((off / tol.clamp(min=1e-300))[bad].max()))
+
+
+# ---- rms_norm -----------------------------------------------------------------------------------------------------------
+def norm_reference(x, r, w, eps):
+    h = x.double() + (0 if r is None else r.double())
+    return h, h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps) * (1 if w is None else w.double())
+
+
+def check_norm(x, r, w, eps, quantize, got):
+    """x, r, w on the host; got: what the operator returned."""
+    h, v = norm_reference(x, r, w, eps)
+    C, t = x.shape[-1], x.dtype
+    # h in fp32 once; the mean's error is halved by the root; then the root's, the weight's and the scale's roundings
+    rel = (2 + (C + 2) / 2 + 8) * 2.0 ** -24 if C < 128 else (2 + (C / 64 + 64) / 2 + 8) * 2.0 ** -24
+    if r is not None:
+        within(got[-1], h, h.abs() * (u(t) + 2.0 ** -24) + TINY[t], "h")
+    if not quantize:
+        y = got[0] if r is not None else got
+        assert y.dtype == t and y.shape == x.shape
+        within(y, v, v.abs() * (u(t) * (1 + rel) + rel) + TINY[t], "y")
+        return
+    q, s = got[0], got[1]
+    assert q.dtype == E4M3 and q.shape == x.shape and s.dtype == F32 and s.shape == x.shape[:-1]
+    top = v.abs().amax(-1)
+    s64 = torch.where(top > 0, (top / 448).clamp(min=2.0 ** -126), torch.ones_like(top))
+    within(s, s64, s64 * (rel + 2.0 ** -23), "scale")
+    back = q.double().cpu() * s.double().cpu().unsqueeze(-1)
+    within(back, v, v.abs() * (2.0 ** -4 + 2 * rel) + s64.unsqueeze(-1) * 2.0 ** -10 * (1 + 1e-5), "q * scale")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("rows,C", [(1, 1), (3, 2), (5, 7), (1, 64), (9, 192), (4, 256), (65, 257), (2, 1000), (3, 1111), (1, 4096), (2, 8192),
+                                    (3, 8200), (2, 16384), (1, 20001), (300, 320), (1025, 16), (2, 70000)])
+def test_rms_norm(dtype, quantize, rows, C):
+    from compression_amd import ops
+    for residual in (False, True):
+        x = rnd(rows * 7 + C, rows, C, scale=3.0).to(dtype)
+        r = rnd(rows + C, rows, C).to(dtype) if residual else None
+        w = 1 + 0.3 * rnd(C, C)
+        got = ops.rms_norm(x.to(DEV), w.to(DEV), 1e-6, None if r is None else r.to(DEV), quantize)
+        check_norm(x, r, w, 1e-6, quantize, got)
+
+
+def test_rms_norm_strides_alignment_and_shapes():
+    from compression_amd import ops
+    for dtype in (F32, F16, BF16):
+        wide = rnd(1, 6, 5, 400).to(dtype)
+        gw = wide.to(DEV)
+        for sl in (slice(0, 192), slice(1, 193), slice(3, 259), slice(8, 264), slice(0, 399)):
+            x, gx = wide[..., sl], gw[..., sl]
+            rr = rnd(2, 6, 5, x.shape[-1]).to(dtype)
+            for quantize in (False, True):
+                check_norm(x, rr, None, 1e-5, quantize, ops.rms_norm(gx, None, 1e-5, rr.to(DEV), quantize))
+                check_norm(rr, x, None, 1e-5, quantize, ops.rms_norm(rr.to(DEV), None, 1e-5, gx, quantize))
+        one = rnd(3, 256).to(dtype)                                       # one row, no leading axis; a broadcast residual
+        check_norm(one, None, None, 1e-6, True, ops.rms_norm(one.to(DEV), quantize=True))
+        x = rnd(4, 7, 256).to(dtype)
+        check_norm(x, one.expand(7, 256), None, 1e-6, False, ops.rms_norm(x.to(DEV), None, 1e-6, one.to(DEV).expand(7, 256)))
+    q, s, h = ops.rms_norm(torch.zeros(0, 8, device=DEV), residual=torch.zeros(0, 8, device=DEV), quantize=True)
+    assert q.shape == (0, 8) and s.shape == (0,) and h.shape == (0, 8)
+
+
+@pytest.mark.parametrize("C", [5, 192, 1111, 4096, 20000])
+def test_rms_norm_special_values(C):
+    """Rows of zeros, tiny rows, a NaN and an infinity: they stay in their row."""
+    from compression_amd import ops
+    x = rnd(C, 7, C)
+    x[1] = 0.0
+    x[2] *= 1e-22
+    x[3, C // 2] = float("nan")
+    x[5, C - 1] = float("inf")
+    w = 1 + 0.1 * rnd(C + 1, C)
+    ok = [0, 1, 2, 4, 6]
+    y = ops.rms_norm(x.to(DEV), w.to(DEV), 1e-6).cpu()
+    q, s = ops.rms_norm(x.to(DEV), w.to(DEV), 1e-6, quantize=True)
+    check_norm(x[ok], None, w, 1e-6, False, y[ok])
+    check_norm(x[ok], None, w, 1e-6, True, (q.float().cpu()[ok].to(E4M3), s.cpu()[ok]))
+    assert float(s[1]) == 1.0 and not bool(q[1].float().any())
+    assert bool(torch.isnan(y[3]).all()) and bool(torch.isnan(q[3].float()).all()) and math.isnan(float(s[3]))
+    assert math.isnan(float(y[5, C - 1])) and not bool(y[5, :C - 1].any()) and math.isnan(float(s[5]))
+
+
+def test_rms_norm_writes_its_rows_only():
+    """Through the C ABI: guards around every output stay as they were."""
+    from compression_amd import _lib
+    from compression_amd._lib import context_for, ptr
+    for C, rows in ((192, 33), (257, 5), (4096, 3)):
+        x = rnd(C, rows, C).to(BF16).to(DEV)
+        h = torch.full((rows + 2, C), 7.0, dtype=BF16, device=DEV)
+        q = torch.full((rows + 2, C), 5, dtype=torch.uint8, device=DEV)
+        s = torch.full((rows + 2,), 3.0, device=DEV)
+        context_for(x.device).call("mpc_rms_norm", ptr(x), C, ptr(x), C, None, rows, C, 1e-6, _lib.MPC_TYPE_BF16, ptr(h[1:]), ptr(q[1:]),
+                                   _lib.MPC_TYPE_E4M3, ptr(s[1:]))
+        check_norm(x.cpu(), x.cpu(), None, 1e-6, True, (q[1:-1].view(E4M3), s[1:-1], h[1:-1]))
+        for t, v in ((h, 7.0), (q, 5), (s, 3.0)):
+            assert bool((t[0] == v).all()) and bool((t[-1] == v).all())
+
+
+# ---- linear ---------------------------------------------------------------------------------------------------------------
+ACTS = {0: "none", 3: "relu", 5: "gelu", 6: "silu"}
+
+
+def act64(v, act):
+    if act == 3:
+        return v.clamp(min=0)
+    if act == 5:
+        return 0.5 * v * torch.special.erfc(-v / math.sqrt(2.0))
+    if act == 6:
+        return v * torch.sigmoid(v)
+    return v
+
+
+def check_linear(x, w, bias, act, res, sx, sw, got, what=""):
+    """All on the same device; the reference is computed there in 64 bits."""
+    X, W = x.double(), w.double()
+    if sx is not None:
+        X, W = X * sx.double().unsqueeze(-1), W * sw.double().unsqueeze(-1)
+    K, out = x.shape[-1], got.dtype
+    Wt = W.t().contiguous()
+    z, mag = X @ Wt, X.abs() @ Wt.abs()
+    off = mag * (K * 2.0 ** -23) + (0 if sx is None else z.abs() * 2.0 ** -22)
+    if sx is not None:
+        # The 8-bit matrix instructions (all four shapes alike, probed with single powers of two beside a product of 2^16)
+        # add the products of eight neighbouring k on a grid of 2^-13 of the largest one's 2^(exponents' sum), cutting
+        # off what lies below, and the eights in fp32.  A product is at least 2^(exponents' sum), and the largest itself,
+        # 6 bits behind its point, is kept whole: the other seven lose less than 2^-13 of it each.
+        off = off + mag * (7 * 2.0 ** -13)
+    if bias is not None:
+        z = z + bias.double()
+        off = off + z.abs() * 2.0 ** -24
+    y = act64(z, act)
+    # slopes of gelu and silu stay below 1.13; their evaluation is good to a few 1e-7 of the argument
+    off = off * 1.13 + (0 if act in (0, 3) else z.abs() * 5e-7)
+    if res is not None:
+        y = y + res.double()
+        off = off + y.abs() * 2.0 ** -24
+    assert got.shape == y.shape
+    within(got, y, off * (1 + u(out)) + y.abs() * u(out) + TINY[out], what)
+
+
+def operands(seed, M, N, K, dtype):
+    x, w = rnd(seed, M, K).to(DEV), (rnd(seed + 1, N, K) / math.sqrt(K)).to(DEV)
+    if dtype != E4M3:
+        return x.to(dtype), w.to(dtype), None, None
+    sx, sw = x.abs().amax(1) / 448, w.abs().amax(1) / 448
+    return (x / sx[:, None]).to(E4M3), (w / sw[:, None]).to(E4M3), sx, sw
+
+
+SIZES = [(1, 1, 1), (1, 64, 64), (1, 1000, 200), (2, 33, 7), (3, 256, 1024), (7, 130, 4096), (15, 64, 129), (16, 512, 512), (17, 100, 333),
+         (31, 320, 192), (33, 192, 320), (63, 65, 66), (64, 256, 256), (65, 1000, 128), (128, 128, 8192), (129, 127, 100), (200, 300, 400),
+         (257, 255, 513), (512, 1024, 256), (1000, 64, 1111), (1537, 1000, 144), (100, 3, 5000), (1, 5, 20000), (640, 640, 72)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_linear(dtype, M, N, K):
+    from compression_amd import ops
+    x, w, sx, sw = operands(M * 3 + N * 5 + K, M, N, K, dtype)
+    i = SIZES.index((M, N, K))
+    odt = (F16, BF16, F32)[i % 3]
+    bias, res = rnd(5, N).to(DEV), rnd(6, M, N).to(odt).to(DEV)
+    for act, b, r in ((0, None, None), (list(ACTS)[i % 4], bias, res), (list(ACTS)[(i + 1) % 4], None, res), (list(ACTS)[(i + 2) % 4], bias, None)):
+        got = ops.linear(x, w, b, act, r, sx, sw, odt)
+        check_linear(x, w, b, act, r, sx, sw, got, (act, b is not None, r is not None))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("M,N,K", SIZES + [(700, 900, 2000), (3, 4096, 4096), (5000, 260, 1030)])
+def test_linear_whole_numbers_exactly(dtype, M, N, K):
+    """Small whole operands: every product and sum is a whole number below 2^24, exact in fp32 and on the 8-bit
+    instructions' grid, so one value of k too many, too few or in the wrong place shows."""
+    from compression_amd import ops
+    g = torch.Generator().manual_seed(M + N + K)
+    x = torch.randint(-8, 9, (M, K), generator=g).float().to(DEV)
+    w = torch.randint(-8, 9, (N, K), generator=g).float().to(DEV)
+    eight = dtype == E4M3
+    sx, sw = (torch.full((M,), 0.5, device=DEV), torch.full((N,), 4.0, device=DEV)) if eight else (None, None)
+    got = ops.linear(x.to(dtype), w.to(dtype), x_scale=sx, weight_scale=sw, out_dtype=F32)
+    want = (x.double() @ w.double().t().contiguous()) * (2.0 if eight else 1.0)
+    assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("M,N,K", [(2100, 2050, 520), (4096, 1024, 256), (8200, 256, 1024), (3000, 4100, 136), (9, 4096, 4096), (300, 4096, 2048),
+                                   (36864, 64, 256), (2048, 2048, 2048), (5000, 1030, 1040)])
+def test_linear_large(dtype, M, N, K):
+    from compression_amd import ops
+    x, w, sx, sw = operands(M + N + K, M, N, K, dtype)
+    bias, res = rnd(7, N).to(DEV), rnd(8, M, N).to(BF16).to(DEV)
+    check_linear(x, w, bias, 5, res, sx, sw, ops.linear(x, w, bias, 5, res, sx, sw, BF16))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("M", [1, 5, 40, 200])
+def test_linear_strides_and_alignment(dtype, M):
+    """Slices of wider rows, rows that start at any element, broadcast rows, leading axes, and no copy of any of them."""
+    from compression_amd import ops
+    K, N = 136, 72
+    x, w, sx, sw = operands(10, M, N, K + 24, dtype)
+    for lo, hi in ((0, K), (1, K + 1), (3, K + 20), (8, K + 8), (16, 21), (0, K + 23)):
+        xs, ws = x[:, lo:hi], w[:, lo:hi]
+        wide = rnd(11, M, N + 11).to(BF16).to(DEV)
+        for r in (None, wide[:, 3:3 + N], wide[:, 8:8 + N]):
+            check_linear(xs, ws, None, 0, r, sx, sw, ops.linear(xs, ws, None, 0, r, sx, sw, BF16), (lo, hi))
+    if M == 40:
+        x3, s3 = x.view(5, 8, -1), None if sx is None else sx.view(5, 8)
+        got = ops.linear(x3, w, None, 3, None, s3, sw, F32)
+        assert got.shape == (5, 8, N)
+        check_linear(x3, w, None, 3, None, s3, sw, got)
+    row = x[:1].expand(M, -1)
+    srow = None if sx is None else sx[:1].expand(M).contiguous()
+    check_linear(row, w, None, 0, None, srow, sw, ops.linear(row, w, None, 0, None, srow, sw, F32))
+    empty = ops.linear(x[:0], w, None, 0, None, None if sx is None else sx[:0], sw, F16)
+    assert empty.shape == (0, N) and empty.dtype == F16
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("M,K", [(1, 100), (6, 1111), (50, 260), (300, 72)])
+def test_linear_special_values_stay_where_they_are(dtype, M, K):
+    """NaN in a row of x or of w reaches that row or column of the output and nothing else: rows and values behind the
+    edges of a tile are never multiplied in, not even by zero."""
+    from compression_amd import ops
+    N = 70
+    x, w, sx, sw = operands(12, M, N, K, dtype)
+    clean = ops.linear(x, w, None, 0, None, sx, sw, F32)
+    pad_x = torch.full((M + 1, K + 9), float("nan"), device=DEV).to(dtype)     # NaN behind every row's end and behind the last row
+    pad_w = torch.full((N + 1, K + 9), float("nan"), device=DEV).to(dtype)
+    pad_x[:M, :K], pad_w[:N, :K] = x, w
+    assert torch.equal(ops.linear(pad_x[:M, :K], pad_w[:N, :K], None, 0, None, sx, sw, F32), clean)
+    xn = pad_x[:M, :K]
+    xn[M // 2, K - 1] = float("nan")
+    got = ops.linear(xn, pad_w[:N, :K], None, 3, None, sx, sw, F32)
+    assert bool(torch.isnan(got[M // 2]).all()) and int(torch.isnan(got).sum()) == N
+    wn = pad_w[:N, :K]
+    wn[N - 1, 0] = float("nan")
+    got = ops.linear(x, wn, None, 0, None, sx, sw, F32)
+    assert bool(torch.isnan(got[:, N - 1]).all()) and torch.equal(got[:, :N - 1], clean[:, :N - 1])
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(1, 100, 256, F16), (20, 70, 4096, BF16), (130, 129, 64, E4M3), (300, 512, 128, BF16)])
+def test_linear_in_place_and_guards(M, N, K, dtype):
+    """Through the C ABI: out may be the residual; what lies behind its rows and columns stays as it was."""
+    import ctypes
+    from compression_amd import _lib
+    from compression_amd._lib import context_for, ptr
+    x, w, sx, sw = operands(13, M, N, K, dtype)
+    for pad in (0, 5, 8):
+        buf = rnd(14, M + 2, N + pad).to(BF16).to(DEV)
+        was = buf.clone()
+        t = {F16: 1, BF16: 2, E4M3: 3}[dtype]
+        d = _lib.LinearDesc(t, _lib.MPC_TYPE_BF16, 6, M, N, K, K, K, N + pad, N + pad)
+        ctx = context_for(x.device)
+        nb = ctx.lib.mpc_linear_workspace_bytes(ctypes.byref(d))
+        work = torch.zeros(max(nb, 16) + 64, dtype=torch.uint8, device=DEV)
+        work[nb:] = 77
+        ctx.call("mpc_linear_forward", ctypes.byref(d), ptr(x), ptr(sx), ptr(w), ptr(sw), None, ptr(buf[1:]), ptr(work), nb, ptr(buf[1:]))
+        check_linear(x, w, None, 6, was[1:-1, :N], sx, sw, buf[1:-1, :N])
+        assert torch.equal(buf[0], was[0]) and torch.equal(buf[-1], was[-1]) and torch.equal(buf[:, N:], was[:, N:])
+        assert bool((work[nb:] == 77).all())
+
+
+def test_linear_repeats_its_bits():
+    from compression_amd import ops
+    for M, N, K in ((1, 1000, 8192), (40, 300, 8192), (300, 300, 4096), (700, 900, 2048)):
+        x, w, _, _ = operands(15, M, N, K, BF16)
+        first = ops.linear(x, w, out_dtype=F32)
+        for _ in range(5):
+            assert torch.equal(ops.linear(x, w, out_dtype=F32), first)
+
+
+# ---- prior_balance ----------------------------------------------------------------------------------------------------------
+def balance_reference(s, scale, k, mask, grad_out=1.0):
+    """-> loss, counts, rows that count, gradient, |gradient| terms: 64 bits, row by row in plain Python order."""
+    v = (s.double() if scale > 0 else -s.double())
+    T, E = v.shape
+    keep = (v > -math.inf).any(1) | torch.isnan(v).any(1)
+    if mask is not None:
+        keep &= mask.bool()
+    p = torch.zeros(T, E, dtype=torch.float64)
+    p[keep] = torch.softmax(v[keep] * abs(scale), 1)
+    order = torch.sort(torch.nan_to_num(v, nan=-math.inf, posinf=math.inf, neginf=-math.inf), dim=1, descending=True, stable=True)
+    counts = torch.zeros(E, dtype=torch.int64)
+    sel = (order.values[:, :k] > -math.inf) & keep[:, None]
+    counts += torch.bincount(order.indices[:, :k][sel], minlength=E)
+    R = int(keep.sum())
+    grad, mag = torch.zeros(T, E, dtype=torch.float64), torch.zeros(T, E, dtype=torch.float64)
+    if R == 0:
+        return 0.0, counts, 0, grad, mag
+    f = counts.double() / (k * R)
+    loss = E * float((f * (p.sum(0) / R)).sum())
+    g = grad_out * scale * E / R
+    c = f - 1 / E
+    grad[keep] = (g * p * (c - (p * c).sum(1, keepdim=True)))[keep]
+    mag[keep] = (abs(g) * p * (c.abs() + (p * c.abs()).sum(1, keepdim=True)))[keep]
+    return loss, counts, R, grad, mag
+
+
+def check_balance(s, scale, k, mask, gs, gmask):
+    from compression_amd import ops
+    loss, counts, R, grad, mag = balance_reference(s, scale, k, mask, 0.37)
+    gl, gc, gn = ops.prior_balance(gs, scale, k, gmask)
+    gg = ops.prior_balance_grad(gs, gc, gn, torch.full((1,), 0.37, device=DEV), scale, k, gmask)
+    assert gc.dtype == torch.int32 and gc.cpu().tolist() == counts.tolist() and gn.cpu().tolist() == [R]
+    assert gl.shape == () and gg.shape == s.shape and gg.dtype == s.dtype
+    z = (s.double() * scale)
+    z = torch.where(torch.isfinite(z), z, torch.zeros_like(z))
+    spread = float((z.amax(1) - z.amin(1)).clamp(max=90).max()) if s.numel() else 0.0    # (beyond 90, p has left fp32)
+    # exp of an argument that is off by 3 roundings, the exponential itself, the row's sum, the division; sums of p over rows
+    rel = (3 * spread + 12 + s.shape[1] / 8) * 2.0 ** -23
+    if math.isnan(loss):
+        assert math.isnan(float(gl))
+    else:
+        assert abs(float(gl) - loss) <= loss * (rel + (s.shape[0] / 64 + 16) * 2.0 ** -24), (float(gl), loss)
+    t = s.dtype
+    within(gg, grad, mag * (2 * rel + 2.0 ** -21) + grad.abs() * u(t) + TINY[t] + 1e-38, "grad")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T,E", [(1, 1), (1, 64), (2, 2), (5, 3), (100, 8), (63, 63), (1536, 64), (77, 65), (300, 100), (64, 128), (50, 200),
+                                 (1000, 256), (9, 512), (33, 1000), (4, 1024), (5000, 16), (20000, 64)])
+def test_prior_balance(dtype, T, E):
+    for by_expert in (False, True):
+        for k in sorted({1, 2, min(8, E), E if E <= 64 else 8} & set(range(1, E + 1))):
+            s = (rnd(T + E + k, T, E, scale=1.5) + rnd(E, E)).to(dtype)
+            mask = torch.rand(T, generator=torch.Generator().manual_seed(T)) < 0.8 if (T + k) % 2 else None
+            g = s.to(DEV)
+            g = g.t().contiguous().t() if by_expert else g
+            check_balance(s, 1.0, k, mask, g, None if mask is None else mask.to(DEV))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("E", [4, 64, 100, 300])
+def test_prior_balance_rows_with_little_in_them(dtype, E):
+    """Masked rows with NaN in them, rows of -infinity, one value above it, the type's lowest value as a mask, equal
+    values, costs (a negative scale) with +infinity as the mask."""
+    low = torch.finfo(dtype).min
+    for sign in (1.0, -1.0):
+        s = (rnd(E, 40, E).to(dtype) * 4).round() / 4                     # many equal values
+        mask = torch.ones(40, dtype=torch.bool)
+        s[0], s[1] = -math.inf, low
+        s[2] = -math.inf
+        s[2, E // 2] = 0.5
+        s[3, 1:] = low
+        s[4] = 0.0
+        s[5], mask[5] = math.nan, False
+        s[6], mask[6] = math.inf, False
+        s[7, ::2] = -math.inf
+        s[8], mask[8] = -math.inf, False
+        s = s * sign
+        for k in (1, 3, 4):
+            for scale in (0.7 * sign, 0.01 * sign):
+                g = s.to(DEV)
+                check_balance(s, scale, k, mask, g, mask.to(DEV))
+                check_balance(s, scale, k, mask, g.t().contiguous().t(), mask.to(torch.uint8).to(DEV))
+
+
+def test_prior_balance_nan_and_no_rows():
+    from compression_amd import ops
+    s = rnd(1, 10, 64)
+    s[3, 7] = math.nan
+    check_balance(s, 1.0, 2, None, s.to(DEV), None)                       # NaN loss, NaN in that row's gradient alone
+    mask = torch.zeros(10, dtype=torch.bool)
+    check_balance(s, 1.0, 2, mask, s.to(DEV), mask.to(DEV))
+    e = torch.zeros(0, 64, device=DEV)
+    loss, counts, n = ops.prior_balance(e)
+    assert float(loss) == 0.0 and int(n) == 0 and not bool(counts.any())
+    assert ops.prior_balance_grad(e, counts, n).shape == (0, 64)
+
+
+def test_prior_balance_strides():
+    from compression_amd import ops
+    wide = rnd(2, 60, 200)
+    for dtype in (F32, BF16):
+        w = wide.to(dtype)
+        gw = w.to(DEV)
+        for s, g in ((w[:, 3:67], gw[:, 3:67]), (w[::3, 8:72], gw[::3, 8:72]), (w[:, ::3], gw[:, ::3]), (w.t()[5:100, :33], gw.t()[5:100, :33]),
+                     (w[:1].expand(9, 200), gw[:1].expand(9, 200))):
+            check_balance(s, 1.3, 2, None, g, None)
+    g = wide.to(DEV).t()
+    loss, counts, n = ops.prior_balance(g)
+    assert ops.prior_balance_grad(g, counts, n).stride() == g.stride()    # the scores' own layout
+
+
+def test_prior_balance_gradient_by_differences():
+    """With the choices held, the loss's central difference in 64 bits gives what the operator returns."""
+    from compression_amd import ops
+    for scale, k in ((0.8, 2), (-0.3, 1)):
+        s = rnd(5, 12, 10, scale=2.0)
+        g = s.to(DEV)
+        loss, counts, n = ops.prior_balance(g, scale, k)
+        grad = ops.prior_balance_grad(g, counts, n, scale=scale, top_k=k).double().cpu()
+        f = counts.double().cpu() / (k * 12)
+
+        def value(t):
+            return 10 * float((f * torch.softmax(t * scale, 1).mean(0)).sum())
+        h = 1e-5
+        for t, j in ((0, 0), (3, 7), (11, 9), (5, 2)):
+            a, b = s.double().clone(), s.double().clone()
+            a[t, j] += h
+            b[t, j] -= h
+            # the difference's own error: h^2 / 6 times a third derivative below 10 / 12, and 2^-52 / h of the loss's size
+            assert abs((value(a) - value(b)) / (2 * h) - float(grad[t, j])) < 1e-6
+
+
+def test_prior_balance_repeats_its_bits():
+    from compression_amd import ops
+    s = rnd(6, 50000, 64).to(DEV)
+    loss, counts, n = ops.prior_balance(s, top_k=2)
+    for _ in range(5):
+        l2, c2, n2 = ops.prior_balance(s, top_k=2)
+        assert torch.equal(loss, l2) and torch.equal(counts, c2)
+
+
+# ---- all of them -----------------------------------------------------------------------------------------------------------
+def test_offsets_beyond_32_bits():
+    """Rows that lie more than 2^32 bytes apart."""
+    from compression_amd import ops
+    step = (1 << 31) + 128                                                # elements of 2 bytes
+    buf = torch.zeros(step + 4096, dtype=BF16, device=DEV)
+    x = torch.as_strided(buf, (2, 320), (step, 1))
+    x.copy_(rnd(20, 2, 320).to(BF16))
+    check_norm(x.cpu(), None, None, 1e-6, False, ops.rms_norm(x))
+    w = (rnd(21, 48, 320) / 18).to(BF16).to(DEV)
+    check_linear(x, w, None, 0, None, None, None, ops.linear(x, w))
+    check_linear(w, x, None, 0, None, None, None, ops.linear(w, x))
+    r = torch.as_strided(buf, (2, 48), (step, 1))
+    check_linear(x, w, None, 0, r, None, None, ops.linear(x, w, residual=r))
+    s = torch.as_strided(buf, (2, 64), (step, 1))
+    check_balance(s.cpu(), 1.0, 2, None, s, None)
+    s = torch.as_strided(buf, (64, 2), (1, step))
+    check_balance(s.cpu(), 1.0, 1, None, s, None)
+
+
+def head(ops, _lib, t):
+    """Scores for the priors from a latent, the way a learned choice would make them: norm, product, product back onto the
+    residual stream, scores, balance and its gradient."""
+    q, sx, h = ops.rms_norm(t["x"], t["g"], residual=t["r"], quantize=True)
+    a = ops.linear(q, t["w1"], t["b1"], _lib.MPC_ACT_GELU, None, sx, t["s1"], BF16)
+    h = ops.linear(a, t["w2"], None, _lib.MPC_ACT_NONE, h)
+    scores = ops.linear(ops.rms_norm(h, t["g"]), t["w3"], out_dtype=F32)
+    loss, counts, n = ops.prior_balance(scores, top_k=1)
+    return scores, loss, counts, ops.prior_balance_grad(scores, counts, n)
+
+
+def head_tensors(seed, rows):
+    C, H, K = 256, 512, 64
+    w1 = rnd(seed + 1, H, C) / 16
+    s1 = w1.abs().amax(1) / 448
+    t = dict(x=rnd(seed, rows, C).to(BF16), r=rnd(seed + 2, rows, C).to(BF16), g=1 + 0.1 * rnd(seed + 3, C), w1=(w1 / s1[:, None]).to(E4M3),
+             s1=s1, b1=rnd(seed + 4, H) * 0.1, w2=(rnd(seed + 5, C, H) / 22).to(BF16), w3=(rnd(seed + 6, K, C) / 16).to(BF16))
+    return {k: v.to(DEV) for k, v in t.items()}
+
+
+@pytest.mark.parametrize("rows", [1, 96, 1536])
+def test_a_head_that_scores_the_priors(rows):
+    from compression_amd import _lib, ops
+    t = head_tensors(30, rows)
+    scores, loss, counts, grad = head(ops, _lib, t)
+    # 64 bits from the same weights; the 8-bit rounding of the norm alone allows 2^-4 a value, averaged over 256 channels
+    h, v = norm_reference(t["x"], t["r"], t["g"], 1e-6)
+    a = act64(v @ (t["w1"].double() * t["s1"].double()[:, None]).t().contiguous() + t["b1"].double(), 5)
+    h = h + a @ t["w2"].double().t().contiguous()
+    _, v = norm_reference(h, None, t["g"], 1e-6)
+    want = v @ t["w3"].double().t().contiguous()
+    assert float((scores.double() - want).norm() / want.norm()) < 2.0 ** -4
+    ref = balance_reference(scores.cpu(), 1.0, 1, None)
+    assert counts.cpu().tolist() == ref[1].tolist() and abs(float(loss) - ref[0]) < 1e-4 * ref[0]
+    assert float((grad.double().cpu() - ref[3]).norm()) <= 1e-4 * float(ref[3].norm()) + 1e-30
+
+
+def test_training_forward_reports_the_balance():
+    """prior_balance=True adds its three values and changes none of the others."""
+    import compression_amd as ca
+    from tests import synth
+    dev = torch.device(DEV)
+    model = ca.init_model("ManyPriors", dev, out_channel_N=192, out_channel_M=256, num_distributions=64)
+    model.load_state_dict(synth.manypriors_state_dict(234))
+    model.train()
+    x = synth.smooth_image(5, 2, 64, 96).to(dev)
+    noise = torch.rand(2, 256, 4, 6, generator=torch.Generator().manual_seed(1)) - 0.5
+    plain, out = model(x, quant_noise=noise), model(x, quant_noise=noise, prior_balance=True)
+    assert set(out) - set(plain) == {"prior_balance", "prior_counts", "prior_balance_grad"}
+    assert torch.equal(plain["reconstructed_image"], out["reconstructed_image"]) and float(plain["bpp"]) == float(out["bpp"])
+    counts, grad = out["prior_counts"], out["prior_balance_grad"]
+    won = torch.bincount(model.last_dist_select.reshape(-1).cpu(), minlength=64)
+    assert counts.cpu().tolist() == won.tolist() and int(counts.sum()) == 48 and tuple(grad.shape) == (48, 64)
+    assert out["used_dists"] == torch.nonzero(counts.cpu()).view(-1).tolist()
+    assert 1.0 - 1e-3 < float(out["prior_balance"]) <= 64.0 and bool(torch.isfinite(grad).all())
+
+
+def test_streams_and_graphs():
+    """The same head on another stream, and captured: replays follow their inputs and equal the eager results, with other
+    work between them; two captured graphs do not disturb each other."""
+    from compression_amd import _lib, ops
+    sets = [head_tensors(40 + 10 * i, r) for i, r in enumerate((300, 5))]
+    eager = [head(ops, _lib, t) for t in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = head(ops, _lib, sets[0])
+    side.synchronize()
+    for a, b in zip(other, eager[0]):
+        assert torch.equal(a, b)
+    graphs, outs = [], []
+    for t in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(head(ops, _lib, t))
+        graphs.append(g)
+    base = [t["x"].clone() for t in sets]
+    for i in range(4):
+        for t, b in zip(sets, base):
+            t["x"].copy_(b * (1 + 0.5 * i))
+        for g in graphs:
+            g.replay()
+        for t, o in zip(sets, outs):
+            for a, b in zip(head(ops, _lib, t), o):
+                assert torch.equal(a, b)
+        torch.cuda.synchronize()
+
+
+def test_refusals():
+    from compression_amd import _lib, ops
+    from compression_amd._lib import MpcError
+    x, w = torch.zeros(4, 64, dtype=F16, device=DEV), torch.zeros(8, 64, dtype=F16, device=DEV)
+    q, qw, s4, s8 = x.to(E4M3), w.to(E4M3), torch.ones(4, device=DEV), torch.ones(8, device=DEV)
+    sc = torch.zeros(4, 8, device=DEV)
+    i32 = torch.zeros(8, dtype=torch.int32, device=DEV)
+    bad = [lambda: ops.rms_norm(x.double()), lambda: ops.rms_norm(q), lambda: ops.rms_norm(x, w[0]), lambda: ops.rms_norm(x, s4),
+           lambda: ops.rms_norm(x, residual=x.float()), lambda: ops.rms_norm(x, residual=x[:2]), lambda: ops.rms_norm(x, residual=x.cpu()),
+           lambda: ops.rms_norm(x.t()), lambda: ops.rms_norm(x, eps=-1.0), lambda: ops.rms_norm(x, eps=math.nan),
+           lambda: ops.linear(x.float(), w.float()), lambda: ops.linear(x, w.to(BF16)), lambda: ops.linear(x, w[:, :32]),
+           lambda: ops.linear(x, w, act=_lib.MPC_ACT_GDN), lambda: ops.linear(x, w, bias=s4), lambda: ops.linear(x, w, bias=s8.half()),
+           lambda: ops.linear(x, w, x_scale=s4, weight_scale=s8), lambda: ops.linear(q, qw), lambda: ops.linear(q, qw, x_scale=s4),
+           lambda: ops.linear(q, qw, x_scale=s8, weight_scale=s8), lambda: ops.linear(x, w, residual=x), lambda: ops.linear(x, w, out_dtype=E4M3),
+           lambda: ops.linear(x, w, residual=sc, out_dtype=F16), lambda: ops.linear(x, w[:0]), lambda: ops.linear(x[:, :0], w[:, :0]),
+           lambda: ops.linear(x, w.cpu()), lambda: ops.linear(x, w[0]), lambda: ops.linear(x, w[:, ::2]), lambda: ops.linear(x.view(4, 8, 8)[:, :3], w[:, :8].contiguous()),
+           lambda: ops.prior_balance(sc.double()), lambda: ops.prior_balance(sc[0]), lambda: ops.prior_balance(sc, top_k=0),
+           lambda: ops.prior_balance(sc, top_k=9), lambda: ops.prior_balance(sc, scale=0.0), lambda: ops.prior_balance(sc, scale=math.inf),
+           lambda: ops.prior_balance(sc, scale=math.nan), lambda: ops.prior_balance(sc, mask=i32[:4]), lambda: ops.prior_balance(sc, mask=torch.ones(5, dtype=torch.bool, device=DEV)),
+           lambda: ops.prior_balance(torch.zeros(2, 1025, device=DEV)), lambda: ops.prior_balance(sc[:, :0]),
+           lambda: ops.prior_balance_grad(sc, i32[:7], i32[:1]), lambda: ops.prior_balance_grad(sc, i32.long(), i32[:1]),
+           lambda: ops.prior_balance_grad(sc, i32, i32[:1], grad_out=s4)]
+    for k, call in enumerate(bad):
+        with pytest.raises(MpcError):
+            call()
+            pytest.fail(f"call {k} of the list was accepted")
