@@ -1,65 +1,266 @@
 // Root-mean-square norm of rows with the residual's addition and, if wanted, an 8-bit output with a scale per row:
 //   h = x + r,  v[c] = h[c] (mean_c h^2 + eps)^(-1/2) w[c],  y = v  or  y = e4m3(v / s), s = max_c |v| / 448.
+//
+// A row is read once: its threads keep h in registers (fp32) across the sum, the largest value and the output.  The kernel
+// moves x, r, h and y once each and does about ten operations a value, so memory bounds it.
 #include "row_ops.h"
 
 namespace {
 
-constexpr int NORM_THREADS = 256;
+constexpr int NORM_MAX_THREADS = 1024;
+constexpr int NORM_MOST = 8;                       // most 16-byte vectors of a row that a thread keeps
 
-template <typename T>
-__global__ __launch_bounds__(NORM_THREADS) void rms_norm_rows_kernel(const T *__restrict__ x, int64_t xs, const T *__restrict__ res,
-                                                                     int64_t rs, const float *__restrict__ weight, int64_t channels,
-                                                                     float eps, T *__restrict__ h_out, T *__restrict__ y,
-                                                                     uint8_t *__restrict__ q, float *__restrict__ scale) {
-    __shared__ float part[NORM_THREADS / 64];
-    __shared__ unsigned upart[NORM_THREADS / 64];
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x;
-    x += row * xs;
-    if (res) res += row * rs;
-    auto at = [&](int64_t c) { return res ? (float)x[c] + (float)res[c] : (float)x[c]; };
+struct NormArgs {
+    const void *x, *res;
+    int64_t xs, rs, rows;
+    int channels;
+    float eps;
+    const float *weight;
+    void *h, *y;
+    float *scale;
+    int group;                                     // threads of a row, a power of two
+};
 
+
+// s = top / 448 for the row's largest |v| (by its bits: the order of non-negative floats, with NaN above infinity)
+__device__ __forceinline__ float row_scale(unsigned top) {
+    const float s = __uint_as_float(top) / E4M3_MAX;
+    return top == 0 ? 1.0f : s < 0x1p-126f ? 0x1p-126f : s;
+}
+
+// VPT vectors of 16 bytes of x per thread: vector i * group + lane of the row, so the group's accesses are consecutive.
+// Rows may start at any element; the last vector of a row may be short.
+template <typename T, int VPT, bool Q>
+__global__ __launch_bounds__(NORM_MAX_THREADS) void rms_norm_kernel(NormArgs a) {
+    constexpr int W = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(W)));
+    typedef vec vec_any __attribute__((aligned(sizeof(T))));
+    typedef float fvec __attribute__((ext_vector_type(4)));
+    typedef fvec fvec_any __attribute__((aligned(4)));
+    typedef unsigned uvec __attribute__((ext_vector_type(W / 4)));
+    typedef uvec uvec_any __attribute__((aligned(1)));
+    __shared__ float part[NORM_MAX_THREADS / 64];
+    __shared__ unsigned upart[NORM_MAX_THREADS / 64];
+
+    const int G = a.group, tid = threadIdx.x, lane = tid & (G - 1);
+    const int64_t at = (int64_t)blockIdx.x * (blockDim.x / G) + tid / G;
+    const bool mine = at < a.rows;                                   // (the last block may have groups without a row)
+    const int64_t row = mine ? at : a.rows - 1;
+    const T *x = (const T *)a.x + row * a.xs, *r = a.res ? (const T *)a.res + row * a.rs : nullptr;
+    const int C = a.channels;
+
+    float v[VPT][W];
     float sum = 0.0f;
-    for (int64_t c = tid; c < channels; c += NORM_THREADS) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int c = (i * G + lane) * W;
+        vec t;
+        if (c + W <= C) {
+            t = *(const vec_any *)(x + c);
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) t[j] = c + j < C ? x[c + j] : (T)0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[i][j] = (float)t[j];
+    }
+    if (r) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * G + lane) * W;
+            vec t;
+            if (c + W <= C) {
+                t = *(const vec_any *)(r + c);
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j) t[j] = c + j < C ? r[c + j] : (T)0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[i][j] += (float)t[j];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) sum += v[i][j] * v[i][j];
+    if (a.h && mine) {
+        T *h = (T *)a.h + row * C;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * G + lane) * W;
+            if (c + W <= C) {
+                vec t;
+#pragma unroll
+                for (int j = 0; j < W; ++j) t[j] = (T)v[i][j];
+                *(vec_any *)(h + c) = t;
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (c + j < C) h[c + j] = (T)v[i][j];
+            }
+        }
+    }
+    for (int off = (G < 64 ? G : 64) / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if (G > 64) {
+        if ((tid & 63) == 0) part[tid >> 6] = sum;
+        __syncthreads();
+        sum = 0.0f;
+        for (int i = 0; i < G / 64; ++i) sum += part[tid / G * (G / 64) + i];
+    }
+    const float inv = 1.0f / sqrtf(sum / (float)C + a.eps);
+
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int c = (i * G + lane) * W;
+        if (a.weight && c + W <= C) {
+#pragma unroll
+            for (int q = 0; q < W; q += 4) {
+                const fvec w = *(const fvec_any *)(a.weight + c + q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i][q + j] = v[i][q + j] * inv * w[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[i][j] = v[i][j] * inv * (a.weight && c + j < C ? a.weight[c + j] : 1.0f);
+        }
+        if constexpr (Q) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const unsigned b = __float_as_uint(v[i][j]) & 0x7fffffffu;   // (past the row's end: 0, or NaN where all of the row is)
+                top = b > top ? b : top;
+            }
+        }
+    }
+    if constexpr (!Q) {
+        if (!mine) return;
+        T *y = (T *)a.y + row * C;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * G + lane) * W;
+            if (c + W <= C) {
+                vec t;
+#pragma unroll
+                for (int j = 0; j < W; ++j) t[j] = (T)v[i][j];
+                *(vec_any *)(y + c) = t;
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (c + j < C) y[c + j] = (T)v[i][j];
+            }
+        }
+    } else {
+        for (int off = (G < 64 ? G : 64) / 2; off > 0; off >>= 1) {
+            const unsigned o = __shfl_xor(top, off, 64);
+            top = o > top ? o : top;
+        }
+        if (G > 64) {
+            if ((tid & 63) == 0) upart[tid >> 6] = top;
+            __syncthreads();
+            for (int i = 0; i < G / 64; ++i) {
+                const unsigned o = upart[tid / G * (G / 64) + i];
+                top = o > top ? o : top;
+            }
+        }
+        if (!mine) return;
+        const float s = row_scale(top), back = 1.0f / s;
+        if (lane == 0) a.scale[row] = s;
+        uint8_t *y = (uint8_t *)a.y + row * C;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * G + lane) * W;
+            uvec t;
+#pragma unroll
+            for (int q = 0; q < W / 4; ++q) {
+                const int lo = e4m3_pack2<false>(v[i][4 * q] * back, v[i][4 * q + 1] * back, 0);
+                t[q] = (unsigned)e4m3_pack2<true>(v[i][4 * q + 2] * back, v[i][4 * q + 3] * back, lo);
+            }
+            if (c + W <= C) {
+                *(uvec_any *)(y + c) = t;
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (c + j < C) y[c + j] = (uint8_t)(t[j / 4] >> (8 * (j % 4)));
+            }
+        }
+    }
+}
+
+// Rows too long for the registers of a block: three passes over x and r, which the L2 holds after the first.
+template <typename T>
+__global__ __launch_bounds__(NORM_MAX_THREADS) void rms_norm_long_kernel(NormArgs a, bool eight) {
+    constexpr int NT = NORM_MAX_THREADS;
+    __shared__ float part[NT / 64];
+    __shared__ unsigned upart[NT / 64];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, C = a.channels;
+    const T *x = (const T *)a.x + row * a.xs, *r = a.res ? (const T *)a.res + row * a.rs : nullptr;
+    auto at = [&](int c) { return r ? (float)x[c] + (float)r[c] : (float)x[c]; };
+    float sum = 0.0f;
+    for (int64_t c = tid; c < C; c += NT) {
         const float h = at(c);
         sum += h * h;
-        if (h_out) h_out[row * channels + c] = (T)h;
+        if (a.h) ((T *)a.h)[row * C + c] = (T)h;
     }
     sum = wave_sum(sum);
     if ((tid & 63) == 0) part[tid >> 6] = sum;
     __syncthreads();
     sum = 0.0f;
-    for (int i = 0; i < NORM_THREADS / 64; ++i) sum += part[i];
-    const float inv = 1.0f / sqrtf(sum / (float)channels + eps);
-    auto value = [&](int64_t c) { return at(c) * inv * (weight ? weight[c] : 1.0f); };
-    if (!q) {
-        for (int64_t c = tid; c < channels; c += NORM_THREADS) y[row * channels + c] = (T)value(c);
+    for (int i = 0; i < NT / 64; ++i) sum += part[i];
+    const float inv = 1.0f / sqrtf(sum / (float)C + a.eps);
+    auto value = [&](int c) { return at(c) * inv * (a.weight ? a.weight[c] : 1.0f); };
+    if (!eight) {
+        for (int64_t c = tid; c < C; c += NT) ((T *)a.y)[row * C + c] = (T)value(c);
         return;
     }
-    // largest |v| by its bits: the order of non-negative floats, with NaN above infinity
     unsigned top = 0;
-    for (int64_t c = tid; c < channels; c += NORM_THREADS) {
-        const unsigned b = __float_as_uint(fabsf(value(c)));
+    for (int64_t c = tid; c < C; c += NT) {
+        const unsigned b = __float_as_uint(value(c)) & 0x7fffffffu;
         top = b > top ? b : top;
     }
     top = wave_max(top);
     if ((tid & 63) == 0) upart[tid >> 6] = top;
     __syncthreads();
     top = 0;
-    for (int i = 0; i < NORM_THREADS / 64; ++i) top = upart[i] > top ? upart[i] : top;
-    float s = __uint_as_float(top) / E4M3_MAX;
-    s = top == 0 ? 1.0f : s < 0x1p-126f ? 0x1p-126f : s;
-    if (tid == 0) scale[row] = s;
-    const float rs_ = 1.0f / s;
-    for (int64_t c = tid; c < channels; c += NORM_THREADS)
-        q[row * channels + c] = (uint8_t)(e4m3_pack2<false>(value(c) * rs_, 0.0f, 0) & 0xff);
+    for (int i = 0; i < NT / 64; ++i) top = upart[i] > top ? upart[i] : top;
+    const float s = row_scale(top), back = 1.0f / s;
+    if (tid == 0) a.scale[row] = s;
+    for (int64_t c = tid; c < C; c += NT) ((uint8_t *)a.y)[row * C + c] = (uint8_t)(e4m3_pack2<false>(value(c) * back, 0.0f, 0) & 0xff);
 }
 
-template <typename T>
-int launch(mpc_ctx *ctx, const void *x, int64_t xs, const void *res, int64_t rs, const float *weight, int64_t rows, int64_t channels,
-           float eps, void *h, void *y, bool eight, float *scale) {
-    rms_norm_rows_kernel<T><<<dim3((unsigned)rows), dim3(NORM_THREADS), 0, ctx->stream>>>(
-        (const T *)x, xs, (const T *)res, rs, weight, channels, eps, (T *)h, eight ? nullptr : (T *)y, eight ? (uint8_t *)y : nullptr, scale);
+// Vectors per thread and threads per row.  Many rows: as few threads as hold the row (up to NORM_MOST vectors each), so that a wave
+// needs no barrier and has many loads in flight.  Few rows (under `full` waves in all): more threads, for latency.
+template <typename T, bool Q>
+int launch(mpc_ctx *ctx, NormArgs a) {
+    constexpr int W = 16 / sizeof(T);
+    const int64_t vectors = mpc_cdiv(a.channels, W);
+    if (vectors > (int64_t)NORM_MOST * NORM_MAX_THREADS) {
+        rms_norm_long_kernel<T><<<dim3((unsigned)a.rows), dim3(NORM_MAX_THREADS), 0, ctx->stream>>>(a, Q);
+        MPC_CHECK_LAUNCH(ctx, "rms_norm_long");
+        return MPC_OK;
+    }
+    constexpr int64_t full = 2048;
+    int vpt = 0, group = 0;
+    int64_t waste = 0;
+    for (int v : {1, 2, 3, 4, NORM_MOST}) {
+        int64_t g = 1;
+        while (g * v < vectors) g *= 2;
+        if (g > NORM_MAX_THREADS) continue;
+        const int64_t lost = g * v - vectors;
+        // a larger vpt must not leave more of its threads' slots empty, and must keep the card full of waves
+        if (group && (lost * 8 > g * v + waste * 8 || a.rows * g < full * 64)) continue;
+        vpt = v, group = (int)g, waste = lost;
+    }
+    a.group = group;
+    const int threads = group > 256 ? group : 256;
+    const dim3 grid((unsigned)mpc_cdiv(a.rows, threads / group)), block(threads);
+    switch (vpt) {
+        case 1: rms_norm_kernel<T, 1, Q><<<grid, block, 0, ctx->stream>>>(a); break;
+        case 2: rms_norm_kernel<T, 2, Q><<<grid, block, 0, ctx->stream>>>(a); break;
+        case 3: rms_norm_kernel<T, 3, Q><<<grid, block, 0, ctx->stream>>>(a); break;
+        case 4: rms_norm_kernel<T, 4, Q><<<grid, block, 0, ctx->stream>>>(a); break;
+        default: rms_norm_kernel<T, NORM_MOST, Q><<<grid, block, 0, ctx->stream>>>(a);
+    }
     MPC_CHECK_LAUNCH(ctx, "rms_norm");
     return MPC_OK;
 }
@@ -72,14 +273,18 @@ extern "C" int mpc_rms_norm(mpc_ctx *ctx, const void *x, int64_t x_stride, const
     MPC_ENTER(ctx);
     MPC_REQUIRE(ctx, type == MPC_TYPE_F32 || type == MPC_TYPE_F16 || type == MPC_TYPE_BF16, "rms_norm: type %d", type);
     MPC_REQUIRE(ctx, y_type == type || y_type == MPC_TYPE_E4M3, "rms_norm: output type %d from type %d", y_type, type);
-    MPC_REQUIRE(ctx, rows >= 0 && rows < (1ll << 31) && channels > 0 && channels < (1ll << 31), "rms_norm: rows = %lld, channels = %lld",
+    MPC_REQUIRE(ctx, rows >= 0 && rows < (1ll << 31) && channels > 0 && channels < (1ll << 31) - 65536, "rms_norm: rows = %lld, channels = %lld",
                 (long long)rows, (long long)channels);
     MPC_REQUIRE(ctx, eps >= 0.0f && eps < INFINITY, "rms_norm: eps = %g", (double)eps);
     if (rows == 0) return MPC_OK;
     const bool eight = y_type == MPC_TYPE_E4M3;
     MPC_REQUIRE(ctx, x && y && (scale != nullptr) == eight, "rms_norm: null pointer, or a scale without an 8-bit output");
     MPC_REQUIRE(ctx, x_stride >= 0 && residual_stride >= 0, "rms_norm: negative stride");
-    if (type == MPC_TYPE_F32) return launch<float>(ctx, x, x_stride, residual, residual_stride, weight, rows, channels, eps, h, y, eight, scale);
-    if (type == MPC_TYPE_F16) return launch<f16_t>(ctx, x, x_stride, residual, residual_stride, weight, rows, channels, eps, h, y, eight, scale);
-    return launch<bf16_t>(ctx, x, x_stride, residual, residual_stride, weight, rows, channels, eps, h, y, eight, scale);
+    const int tb = mpc_type_bytes(type);
+    MPC_REQUIRE(ctx, ((uintptr_t)x | (uintptr_t)residual | (uintptr_t)h | (eight ? 0 : (uintptr_t)y)) % tb == 0 &&
+                         ((uintptr_t)weight | (uintptr_t)scale) % 4 == 0, "rms_norm: misaligned pointer");
+    const NormArgs a{x, residual, x_stride, residual_stride, rows, (int)channels, eps, weight, h, y, scale, 0};
+    if (type == MPC_TYPE_F32) return eight ? launch<float, true>(ctx, a) : launch<float, false>(ctx, a);
+    if (type == MPC_TYPE_F16) return eight ? launch<f16_t, true>(ctx, a) : launch<f16_t, false>(ctx, a);
+    return eight ? launch<bf16_t, true>(ctx, a) : launch<bf16_t, false>(ctx, a);
 }
