@@ -187,13 +187,15 @@ class Context:
             raise MpcError(f"mpc_create(device {device_index}) failed with {rc}: no usable MI355X / HIP runtime")
         self.handle = h
         self.device_index = device_index
+        self.stream_handle = stream_handle
         register_owner(self)
 
     def set_stream(self, stream_handle: int):
         self.check(self.lib.mpc_set_stream(self.handle, c_void_p(stream_handle)))
+        self.stream_handle = stream_handle
 
     def check(self, rc: int):
-        if rc:
+        if rc != 0:
             msg = self.lib.mpc_last_error(self.handle)
             raise MpcError(f"libmpc error {rc}: {msg.decode() if msg else ''}")
 
@@ -225,5 +227,7 @@ def context_for(device) -> Context:
     ctx = _contexts.get(index)
     if ctx is None:
         ctx = _contexts[index] = Context(index, 0)
-    ctx.set_stream(torch.cuda.current_stream(index).cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(index)     # (what torch.cuda.current_stream(index).cuda_stream is, without the object)
+    if stream != ctx.stream_handle:
+        ctx.set_stream(stream)
     return ctx

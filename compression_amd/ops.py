@@ -312,6 +312,20 @@ def _same_gpu(x: torch.Tensor, **others):
             raise MpcError(f"{name} is on {t.device}, the input on {x.device}")
 
 
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _call(name: str, device, entry: str, *args, **meta):
+    """One library call, timed under `name` if a Profiler is on (its context manager costs as much as the launch of a small
+    call, so it is left out otherwise)."""
+    if PROFILER is None:
+        context_for(device).call(entry, *args)
+    else:
+        with _timed(name, **meta):
+            context_for(device).call(entry, *args)
+
+
 def _vector(t: Optional[torch.Tensor], n: int, name: str):
     if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
         raise MpcError(f"{name} must be {n} contiguous float32 values, got {t.dtype} {tuple(t.shape)}")
@@ -342,9 +356,9 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quantize else None
     t = _ROW_TYPES[x.dtype]
     if rows:
-        with _timed("rms_norm", bytes=float(x.numel()) * (x.element_size() * (1 if residual is None else 3) + y.element_size())):
-            context_for(x.device).call("mpc_rms_norm", ptr(x), xs, ptr(residual), rs, ptr(weight), rows, C, float(eps), t, ptr(h), ptr(y),
-                                       _lib.MPC_TYPE_E4M3 if quantize else t, ptr(scale))
+        _call("rms_norm", x.device, "mpc_rms_norm", x.data_ptr(), xs, _addr(residual), rs, _addr(weight), rows, C, eps, t, _addr(h),
+              y.data_ptr(), _lib.MPC_TYPE_E4M3 if quantize else t, _addr(scale),
+              bytes=float(x.numel()) * (x.element_size() * (1 if residual is None else 3) + y.element_size()))
     out = ((y, scale) if quantize else (y,)) + (() if h is None else (h,))
     return out if len(out) > 1 else y
 
@@ -387,12 +401,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         return out
     K = x.shape[-1]
     desc = _lib.LinearDesc(_OPERAND_TYPES[x.dtype], _ROW_TYPES[odt], act, M, N, K, xs, ws, rs, N)
-    ctx = context_for(x.device)
-    ws_bytes = ctx.lib.mpc_linear_workspace_bytes(ctypes.byref(desc))
+    ws_bytes = _lib.load().mpc_linear_workspace_bytes(desc)
     work = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    with _timed("linear", flops=2.0 * M * N * K):
-        ctx.call("mpc_linear_forward", ctypes.byref(desc), ptr(x), ptr(x_scale), ptr(weight), ptr(weight_scale), ptr(bias), ptr(residual),
-                 ptr(work), ws_bytes, ptr(out))
+    _call("linear", x.device, "mpc_linear_forward", desc, x.data_ptr(), _addr(x_scale), weight.data_ptr(), _addr(weight_scale), _addr(bias),
+          _addr(residual), _addr(work), ws_bytes, out.data_ptr(), flops=2.0 * M * N * K)
     return out
 
 
@@ -403,7 +415,7 @@ def _balance_args(scores, scale, top_k, mask):
     T, E = scores.shape
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (T,) or not mask.is_contiguous()):
         raise MpcError(f"prior_balance: mask must be {T} contiguous bool values, got {mask.dtype} {tuple(mask.shape)}")
-    return (ptr(scores), _ROW_TYPES[scores.dtype], T, E, scores.stride(0), scores.stride(1), float(scale), int(top_k), ptr(mask))
+    return (scores.data_ptr(), _ROW_TYPES[scores.dtype], T, E, scores.stride(0), scores.stride(1), scale, top_k, _addr(mask))
 
 
 def prior_balance(scores: torch.Tensor, scale: float = 1.0, top_k: int = 1, mask: Optional[torch.Tensor] = None):
@@ -420,11 +432,10 @@ def prior_balance(scores: torch.Tensor, scale: float = 1.0, top_k: int = 1, mask
     loss = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty(E, dtype=torch.int32, device=dev)
     n_rows = torch.empty(1, dtype=torch.int32, device=dev)
-    ctx = context_for(dev)
-    ws_bytes = ctx.lib.mpc_prior_balance_workspace_bytes(T, E)
+    ws_bytes = _lib.load().mpc_prior_balance_workspace_bytes(T, E)
     work = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with _timed("prior_balance", bytes=float(scores.numel()) * scores.element_size()):
-        ctx.call("mpc_prior_balance", *args, ptr(work), ws_bytes, ptr(loss), ptr(counts), ptr(n_rows))
+    _call("prior_balance", dev, "mpc_prior_balance", *args, work.data_ptr(), ws_bytes, loss.data_ptr(), counts.data_ptr(), n_rows.data_ptr(),
+          bytes=float(scores.numel()) * scores.element_size())
     return loss, counts, n_rows
 
 
@@ -441,9 +452,8 @@ def prior_balance_grad(scores: torch.Tensor, counts: torch.Tensor, n_rows: torch
             raise MpcError(f"prior_balance_grad: {name} must be {n} contiguous int32 values, got {t.dtype} {tuple(t.shape)}")
     _vector(grad_out, 1, "grad_out")
     grad = torch.empty_like(scores)
-    with _timed("prior_balance_grad", bytes=2.0 * scores.numel() * scores.element_size()):
-        context_for(scores.device).call("mpc_prior_balance_grad", *args, ptr(counts), ptr(n_rows), ptr(grad_out), ptr(grad), grad.stride(0),
-                                        grad.stride(1))
+    _call("prior_balance_grad", scores.device, "mpc_prior_balance_grad", *args, counts.data_ptr(), n_rows.data_ptr(), _addr(grad_out),
+          grad.data_ptr(), grad.stride(0), grad.stride(1), bytes=2.0 * scores.numel() * scores.element_size())
     return grad
 
 
