@@ -1,15 +1,19 @@
 // The balance loss of a competition and its gradient.  With z = scale * scores, p = softmax(z) over the experts of a row
 // that counts and f the share of the top_k choices that fell on an expert:
 //   loss = E sum_e f_e mean_t p_te,     d loss / d score_tj = scale E / R p_tj (f_j - sum_e f_e p_te).
-// One wave takes a row: lane l holds experts l, l + 64, ...  A block's waves add up p and the choices of their rows in
-// registers; the blocks' sums meet in a second kernel, in a fixed order and in double.
+//
+// A row belongs to a group of `group` lanes (a power of two), EPL consecutive experts a lane, so that the softmax's and the
+// choice's reductions are a few DPP steps and a wave takes 64 / group rows at once (64 experts: 8 lanes, 8 rows).  A
+// wave keeps the sums of p of its rows in registers and counts choices in LDS; the blocks' sums meet in a second kernel,
+// in a fixed order and in double.  Scores whose experts are not consecutive (the competition writes its totals prior by
+// prior) go through an LDS tile, read and, for the gradient, written along the rows.
 #include "row_ops.h"
 
 namespace {
 
-constexpr int PB_WAVES = 4;
-constexpr int PB_MAX_BLOCKS = 512;
 constexpr int PB_MAX_EXPERTS = 1024;
+constexpr int PB_MAX_THREADS = 512;
+constexpr int PB_MAX_BLOCKS = 512;
 
 struct Row {
     const void *scores;
@@ -18,174 +22,393 @@ struct Row {
     float scale;
     int top_k;
     const uint8_t *mask;
+    int group, group_log2;
+    int tile_rows;                    // staged kernels: rows of an LDS tile (a power of two)
+    int tile_log2;
 };
 
-// v[i] = scores in the order of the choice (costs negated), -inf past the last expert; p[i] the row's softmax.
-// Returns whether the row counts.
-template <typename T, int NI>
-__device__ __forceinline__ bool load_row(const Row &a, int64_t row, int lane, float (&v)[NI], float (&p)[NI]) {
-    if (a.mask && !a.mask[row]) return false;
-    const T *s = (const T *)a.scores + row * a.row_stride;
-    const float mag = fabsf(a.scale);
-    float top = -INFINITY;
-    int nan = 0;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int e = lane + 64 * i;
-        float x = -INFINITY;
-        if (e < a.experts) x = (float)s[e * a.expert_stride];
-        v[i] = e < a.experts && a.scale < 0.0f ? -x : x;
-        nan |= v[i] != v[i];
-        top = fmaxf(top, v[i]);
-    }
-    top = wave_max(top);
-    if (top == -INFINITY && __ballot(nan) == 0) return false;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        p[i] = __expf((v[i] - top) * mag);
-        sum += p[i];
-    }
-    const float inv = 1.0f / wave_sum(sum);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) p[i] *= inv;
-    return true;
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, false);
 }
 
-// partial sums of a block: [block][2 * experts + 1] words: sum of p (float), choices (int), rows (int)
-template <typename T, int NI>
-__global__ __launch_bounds__(64 * PB_WAVES) void prior_balance_kernel(Row a, float *__restrict__ ws) {
-    __shared__ float psum[PB_WAVES][NI * 64];
-    __shared__ int csum[PB_WAVES][NI * 64];
-    __shared__ int rsum[PB_WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float acc[NI];
-    int cnt[NI], n = 0;
+// op over the lanes of a group; every lane gets the result.  Lane i of a quad with i ^ 1, with i ^ 2, then the mirror
+// images of eight and of sixteen lanes.
+template <typename T, typename Op>
+__device__ __forceinline__ T group_reduce(T v, int group, Op op) {
+    if (group > 1) v = op(v, dpp<0xB1>(v));
+    if (group > 2) v = op(v, dpp<0x4E>(v));
+    if (group > 4) v = op(v, dpp<0x141>(v));
+    if (group > 8) v = op(v, dpp<0x140>(v));
+    if (group > 16) v = op(v, __shfl_xor(v, 16, 64));
+    if (group > 32) v = op(v, __shfl_xor(v, 32, 64));
+    return v;
+}
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Min {
+    __device__ __forceinline__ int operator()(int a, int b) const { return a < b ? a : b; }
+};
+struct Add {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct Or {
+    __device__ __forceinline__ int operator()(int a, int b) const { return a | b; }
+};
+
+// A row's values in the order of the choice (costs negated), -inf past the last expert; all 0 if the row does not count.
+template <typename T, int EPL>
+__device__ __forceinline__ void load_values(const Row &a, const T *s, int e0, bool keep, float (&v)[EPL]) {
+    constexpr int W = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(W)));
+    typedef vec vec_any __attribute__((aligned(sizeof(T))));
 #pragma unroll
-    for (int i = 0; i < NI; ++i) acc[i] = 0.0f, cnt[i] = 0;
-    for (int64_t row = (int64_t)blockIdx.x * PB_WAVES + wave; row < a.rows; row += (int64_t)gridDim.x * PB_WAVES) {
-        float v[NI], p[NI];
-        if (!load_row<T, NI>(a, row, lane, v, p)) continue;
-        ++n;
+    for (int i = 0; i < EPL; i += W) {
+        if (e0 + i + W <= a.experts) {
+            const vec t = *(const vec_any *)(s + e0 + i);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) acc[i] += p[i];
-        for (int k = 0; k < a.top_k; ++k) {
-            float best = -INFINITY;
-            int at = PB_MAX_EXPERTS;
+            for (int j = 0; j < W; ++j) v[i + j] = (float)t[j];
+        } else {
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-                if (v[i] > best) best = v[i], at = lane + 64 * i;
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) {
-                const float b = __shfl_xor(best, off, 64);
-                const int o = __shfl_xor(at, off, 64);
-                if (b > best || (b == best && o < at)) best = b, at = o;
-            }
-            if (at == PB_MAX_EXPERTS) break;                 // nothing above -inf is left
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
-                if (at == lane + 64 * i) ++cnt[i], v[i] = -INFINITY;
+            for (int j = 0; j < W; ++j) v[i + j] = e0 + i + j < a.experts ? (float)s[e0 + i + j] : a.scale < 0.0f ? INFINITY : -INFINITY;
         }
     }
 #pragma unroll
-    for (int i = 0; i < NI; ++i) psum[wave][lane + 64 * i] = acc[i], csum[wave][lane + 64 * i] = cnt[i];
+    for (int j = 0; j < EPL; ++j) v[j] = keep ? (a.scale < 0.0f ? -v[j] : v[j]) : 0.0f;
+}
+template <int EPL>
+__device__ __forceinline__ void load_staged(const Row &a, const float *tile_row, int e0, bool keep, float (&v)[EPL]) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        const float x = e0 + j < a.experts ? tile_row[e0 + j] : a.scale < 0.0f ? INFINITY : -INFINITY;
+        v[j] = keep ? (a.scale < 0.0f ? -x : x) : 0.0f;
+    }
+}
+
+// v -> p = e * inv.  Returns whether the row counts (inv = 0 if not).  Changes v only in rows without anything above -inf.
+template <int EPL>
+__device__ __forceinline__ bool softmax(const Row &a, bool keep, float (&v)[EPL], float (&e)[EPL], float &top, float &inv) {
+    const float slope = fabsf(a.scale) * 1.44269504f;
+    top = v[0];
+#pragma unroll
+    for (int j = 1; j < EPL; ++j) top = fmaxf(top, v[j]);
+    top = group_reduce(top, a.group, Max());
+    if (__any(keep && top == -INFINITY)) {                    // rows of -inf (and NaN): rare
+        int nan = 0;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) nan |= v[j] != v[j];
+        nan = group_reduce(nan, a.group, Or());
+        if (top == -INFINITY && !nan) {
+            keep = false;
+            top = 0.0f;
+        }
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        e[j] = __builtin_amdgcn_exp2f((v[j] - top) * slope);
+        sum += e[j];
+    }
+    sum = group_reduce(sum, a.group, Add());
+    inv = keep ? 1.0f / sum : 0.0f;
+    return keep;
+}
+
+// Copies rows [first, first + tile_rows) to LDS, along the rows; rows behind the last become 0.
+template <typename T>
+__device__ __forceinline__ void stage(const Row &a, int64_t first, float *tile) {
+    const int pitch = a.experts + 1;
+    for (int i = threadIdx.x; i < a.experts << a.tile_log2; i += blockDim.x) {
+        const int r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
+        tile[r * pitch + e] = first + r < a.rows ? (float)((const T *)a.scores)[(first + r) * a.row_stride + e * a.expert_stride] : 0.0f;
+    }
+}
+
+// words of a block in the workspace: sum of p (float) [experts], choices (int) [experts], rows (int)
+template <typename T, int EPL, bool STAGED>
+__global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_kernel(Row a, float *__restrict__ ws) {
+    extern __shared__ float lds[];                            // [experts] choices | sums of the waves, or the tile
+    __shared__ int rsum[PB_MAX_THREADS / 64];
+    int *hist = (int *)lds;
+    float *tile = lds + a.experts;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int e0 = (lane & (a.group - 1)) * EPL, per_wave = 64 >> a.group_log2, per_block = per_wave * waves;
+    for (int e = tid; e < a.experts; e += blockDim.x) hist[e] = 0;
+    __syncthreads();
+    float acc[EPL];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) acc[j] = 0.0f;
+
+    auto one = [&](int64_t row, const float *tile_row) {
+        const bool in = row < a.rows;
+        const int64_t at = in ? row : 0;                      // (a group without a row reads row 0 and counts nothing)
+        bool keep = in && (!a.mask || a.mask[at]);
+        float v[EPL], e[EPL], top, inv;
+        if constexpr (STAGED) load_staged<EPL>(a, tile_row, e0, keep, v);
+        else load_values<T, EPL>(a, (const T *)a.scores + at * a.row_stride, e0, keep, v);
+        keep = softmax<EPL>(a, keep, v, e, top, inv);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] = fmaf(keep ? e[j] : 0.0f, inv, acc[j]);
+        n += (int)__popcll(__ballot(keep && e0 == 0));
+        for (int k = 0; k < a.top_k; ++k) {
+            float best = top;
+            if (k > 0) {
+                best = v[0];
+#pragma unroll
+                for (int j = 1; j < EPL; ++j) best = fmaxf(best, v[j]);
+                best = group_reduce(best, a.group, Max());
+            }
+            int at_e = PB_MAX_EXPERTS;
+#pragma unroll
+            for (int j = EPL - 1; j >= 0; --j) at_e = v[j] == best ? e0 + j : at_e;
+            at_e = group_reduce(at_e, a.group, Min());
+            if (keep && best > -INFINITY && e0 == 0) atomicAdd(&hist[at_e], 1);
+            if (k + 1 < a.top_k) {
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) v[j] = e0 + j == at_e ? -INFINITY : v[j];
+            }
+        }
+    };
+    if constexpr (STAGED) {
+        for (int64_t first = (int64_t)blockIdx.x * a.tile_rows; first < a.rows; first += (int64_t)gridDim.x * a.tile_rows) {
+            __syncthreads();                                  // the previous tile has been read
+            stage<T>(a, first, tile);
+            __syncthreads();
+            for (int r = wave * per_wave; r < a.tile_rows; r += per_block) {
+                const int mine = r + (lane >> a.group_log2);  // (tile_rows may be less than a wave's rows)
+                const bool in = mine < a.tile_rows;
+                one(in ? first + mine : a.rows, tile + (in ? mine : 0) * (a.experts + 1));
+            }
+        }
+        __syncthreads();
+    } else {
+        for (int64_t first = (int64_t)blockIdx.x * per_block + wave * per_wave; first < a.rows; first += (int64_t)gridDim.x * per_block)
+            one(first + (lane >> a.group_log2), nullptr);
+    }
+
+    // the groups of a wave, then the waves of the block
+    const int width = a.group * EPL;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+        for (int off = a.group; off < 64; off <<= 1) acc[j] += __shfl_xor(acc[j], off, 64);
+        if (lane < a.group) tile[wave * width + e0 + j] = acc[j];
+    }
     if (lane == 0) rsum[wave] = n;
     __syncthreads();
     float *out = ws + (int64_t)blockIdx.x * (2 * a.experts + 1);
-    for (int e = threadIdx.x; e < a.experts; e += 64 * PB_WAVES) {
+    for (int e = tid; e < a.experts; e += blockDim.x) {
         float s = 0.0f;
-        int c = 0;
-        for (int w = 0; w < PB_WAVES; ++w) s += psum[w][e], c += csum[w][e];
+        for (int w = 0; w < waves; ++w) s += tile[w * width + e];
         out[e] = s;
-        ((int *)out)[a.experts + e] = c;
+        ((int *)out)[a.experts + e] = hist[e];
     }
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         int c = 0;
-        for (int w = 0; w < PB_WAVES; ++w) c += rsum[w];
+        for (int w = 0; w < waves; ++w) c += rsum[w];
         ((int *)out)[2 * a.experts] = c;
     }
 }
 
-__global__ __launch_bounds__(1024) void prior_balance_join_kernel(const float *__restrict__ ws, int blocks, int experts, int top_k,
+// 1024 threads: `slices` of them add up the blocks of one expert
+__global__ __launch_bounds__(1024) void prior_balance_join_kernel(const float *__restrict__ ws, int blocks, int experts, int slices, int top_k,
                                                                   float *__restrict__ loss, int32_t *__restrict__ counts,
                                                                   int32_t *__restrict__ n_rows) {
-    __shared__ double part[16];
-    const int e = threadIdx.x, words = 2 * experts + 1;
+    __shared__ double psum[1024];
+    __shared__ int csum[1024];
+    __shared__ int nsum[16];
+    const int tid = threadIdx.x, words = 2 * experts + 1;
     int n = 0;
-    for (int b = 0; b < blocks; ++b) n += ((const int *)ws)[(int64_t)b * words + 2 * experts];
-    double term = 0.0;
-    if (e < experts) {
-        double p = 0.0;
-        int c = 0;
-        for (int b = 0; b < blocks; ++b) {
+    for (int b = tid; b < blocks; b += 1024) n += ((const int *)ws)[(int64_t)b * words + 2 * experts];
+    for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+    if ((tid & 63) == 0) nsum[tid >> 6] = n;
+    const int slice = tid / experts, e = tid - slice * experts;
+    double p = 0.0;
+    int c = 0;
+    if (slice < slices) {
+#pragma unroll 4
+        for (int b = slice; b < blocks; b += slices) {
             p += (double)ws[(int64_t)b * words + e];
             c += ((const int *)ws)[(int64_t)b * words + experts + e];
         }
-        counts[e] = c;
+    }
+    psum[tid] = p;
+    csum[tid] = c;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < 16; ++w) n += nsum[w];
+    double term = 0.0;
+    if (tid < experts) {
+        for (int s = 1; s < slices; ++s) p += psum[s * experts + tid], c += csum[s * experts + tid];
+        counts[tid] = c;
         if (n > 0) term = (double)c / ((double)top_k * n) * (p / n);
     }
-    for (int off = 32; off > 0; off >>= 1) term += __shfl_xor(term, off, 64);
-    if ((e & 63) == 0) part[e >> 6] = term;
     __syncthreads();
-    if (e == 0) {
+    for (int off = 32; off > 0; off >>= 1) term += __shfl_xor(term, off, 64);
+    if ((tid & 63) == 0) psum[tid >> 6] = term;
+    __syncthreads();
+    if (tid == 0) {
         double s = 0.0;
-        for (unsigned w = 0; w < blockDim.x / 64; ++w) s += part[w];
+        for (int w = 0; w < 16; ++w) s += psum[w];
         *loss = (float)(experts * s);
         *n_rows = n;
     }
 }
 
-template <typename T, int NI>
-__global__ __launch_bounds__(64 * PB_WAVES) void prior_balance_grad_kernel(Row a, const int32_t *__restrict__ counts,
-                                                                           const int32_t *__restrict__ n_rows,
-                                                                           const float *__restrict__ grad_out, T *__restrict__ grad,
-                                                                           int64_t grs, int64_t ges) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <typename T, int EPL, bool STAGED>
+__global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_grad_kernel(Row a, const int32_t *__restrict__ counts,
+                                                                            const int32_t *__restrict__ n_rows,
+                                                                            const float *__restrict__ grad_out, T *__restrict__ grad,
+                                                                            int64_t grs, int64_t ges) {
+    extern __shared__ float tile[];
+    constexpr int W = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(W)));
+    typedef vec vec_any __attribute__((aligned(sizeof(T))));
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int e0 = (lane & (a.group - 1)) * EPL, per_wave = 64 >> a.group_log2, per_block = per_wave * waves;
     const int n = *n_rows;
     // f_j - 1 / E: the difference f_j - sum_e f_e p_te is the same, and loses less where use is nearly even
-    float f[NI];
+    float f[EPL];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int e = lane + 64 * i;
-        f[i] = e < a.experts && n > 0 ? (float)((double)counts[e] / ((double)a.top_k * n) - 1.0 / a.experts) : 0.0f;
-    }
+    for (int j = 0; j < EPL; ++j)
+        f[j] = e0 + j < a.experts && n > 0 ? (float)((double)counts[e0 + j] / ((double)a.top_k * n) - 1.0 / a.experts) : 0.0f;
     const float g = n > 0 ? (float)((double)(grad_out ? *grad_out : 1.0f) * a.scale * a.experts / n) : 0.0f;
-    for (int64_t row = (int64_t)blockIdx.x * PB_WAVES + wave; row < a.rows; row += (int64_t)gridDim.x * PB_WAVES) {
-        float v[NI], p[NI], d = 0.0f;
-        const bool counted = load_row<T, NI>(a, row, lane, v, p);
-        if (counted) {
+
+    auto one = [&](int64_t row, bool in, float *tile_row) {
+        const int64_t at = in ? row : 0;
+        bool keep = in && (!a.mask || a.mask[at]);
+        float v[EPL], e[EPL], top, inv;
+        if constexpr (STAGED) load_staged<EPL>(a, tile_row, e0, keep, v);
+        else load_values<T, EPL>(a, (const T *)a.scores + at * a.row_stride, e0, keep, v);
+        keep = softmax<EPL>(a, keep, v, e, top, inv);
+        float d = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) d += p[i] * f[i];
-            d = wave_sum(d);
+        for (int j = 0; j < EPL; ++j) {
+            e[j] = keep ? e[j] * inv : 0.0f;
+            d = fmaf(e[j], f[j], d);
         }
+        d = group_reduce(d, a.group, Add());
+        const float gk = keep ? g : 0.0f;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int e = lane + 64 * i;
-            if (e < a.experts) grad[row * grs + e * ges] = (T)(counted ? g * p[i] * (f[i] - d) : 0.0f);
+        for (int j = 0; j < EPL; ++j) e[j] *= gk * (f[j] - d);
+        if (!in) return;
+        if constexpr (STAGED) {
+#pragma unroll
+            for (int j = 0; j < EPL; ++j)
+                if (e0 + j < a.experts) tile_row[e0 + j] = e[j];
+        } else {
+            T *o = grad + row * grs;
+            if (ges == 1) {
+#pragma unroll
+                for (int i = 0; i < EPL; i += W) {
+                    if (e0 + i + W <= a.experts) {
+                        vec t;
+#pragma unroll
+                        for (int j = 0; j < W; ++j) t[j] = (T)e[i + j];
+                        *(vec_any *)(o + e0 + i) = t;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < W; ++j)
+                            if (e0 + i + j < a.experts) o[e0 + i + j] = (T)e[i + j];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < EPL; ++j)
+                    if (e0 + j < a.experts) o[(e0 + j) * ges] = (T)e[j];
+            }
+        }
+    };
+    if constexpr (STAGED) {
+        const int pitch = a.experts + 1;
+        for (int64_t first = (int64_t)blockIdx.x * a.tile_rows; first < a.rows; first += (int64_t)gridDim.x * a.tile_rows) {
+            __syncthreads();
+            stage<T>(a, first, tile);
+            __syncthreads();
+            for (int r = wave * per_wave; r < a.tile_rows; r += per_block) {
+                const int mine = r + (lane >> a.group_log2);
+                const bool in = mine < a.tile_rows;
+                one(first + mine, in && first + mine < a.rows, tile + (in ? mine : 0) * pitch);
+            }
+            __syncthreads();
+            for (int i = tid; i < a.experts << a.tile_log2; i += blockDim.x) {
+                const int r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
+                if (first + r < a.rows) grad[(first + r) * grs + e * ges] = (T)tile[r * pitch + e];
+            }
+        }
+    } else {
+        for (int64_t first = (int64_t)blockIdx.x * per_block + wave * per_wave; first < a.rows; first += (int64_t)gridDim.x * per_block) {
+            const int64_t row = first + (lane >> a.group_log2);
+            one(row, row < a.rows, nullptr);
         }
     }
 }
 
-int blocks_for(int64_t rows) {
-    const int64_t b = mpc_cdiv(rows, PB_WAVES);
-    return (int)(b < 1 ? 1 : b > PB_MAX_BLOCKS ? PB_MAX_BLOCKS : b);
+struct Shape {
+    int epl, threads;
+    int64_t passes;                   // blocks that would take every row at once
+    size_t tile_bytes;
+};
+
+// Lanes per row, rows per tile, threads per block.  Few rows: small blocks, so that more CUs take part.
+Shape shape(Row &a, bool staged) {
+    Shape s{};
+    s.epl = a.experts > 8 * 64 ? 16 : 8;
+    a.group = 1, a.group_log2 = 0;
+    while (a.group * s.epl < a.experts) a.group *= 2, ++a.group_log2;
+    const bool few = a.rows <= 64 * 256;
+    int per_block;
+    if (staged) {
+        int r = few ? 16 : 64;
+        while (r > 8 && r * (a.experts + 1) > 12288) r /= 2;
+        a.tile_rows = r;
+        a.tile_log2 = __builtin_ctz(r);
+        const int t = r * a.group;
+        s.threads = t < 128 ? 128 : t > PB_MAX_THREADS ? PB_MAX_THREADS : t;
+        s.tile_bytes = (size_t)r * (a.experts + 1) * sizeof(float);
+        per_block = r;
+    } else {
+        s.threads = few ? 128 : PB_MAX_THREADS;
+        per_block = s.threads / a.group;
+    }
+    s.passes = a.rows > 0 ? mpc_cdiv(a.rows, per_block) : 1;
+    return s;
 }
 
-template <typename T, int NI>
-int forward(mpc_ctx *ctx, const Row &a, float *ws, float *loss, int32_t *counts, int32_t *n_rows) {
-    const int blocks = blocks_for(a.rows);
-    prior_balance_kernel<T, NI><<<dim3(blocks), dim3(64 * PB_WAVES), 0, ctx->stream>>>(a, ws);
+template <typename T>
+int forward(mpc_ctx *ctx, Row a, float *ws, float *loss, int32_t *counts, int32_t *n_rows) {
+    const bool staged = a.expert_stride != 1 && a.experts > 1;
+    const Shape s = shape(a, staged);
+    const int blocks = (int)(s.passes > PB_MAX_BLOCKS ? PB_MAX_BLOCKS : s.passes);
+    size_t sums = (size_t)(s.threads / 64) * a.group * s.epl * sizeof(float);
+    if (sums < s.tile_bytes) sums = s.tile_bytes;
+    const size_t lds = a.experts * sizeof(int) + sums;
+    const dim3 grid(blocks), block(s.threads);
+    if (s.epl == 8 && !staged) prior_balance_kernel<T, 8, false><<<grid, block, lds, ctx->stream>>>(a, ws);
+    if (s.epl == 8 && staged) prior_balance_kernel<T, 8, true><<<grid, block, lds, ctx->stream>>>(a, ws);
+    if (s.epl == 16 && !staged) prior_balance_kernel<T, 16, false><<<grid, block, lds, ctx->stream>>>(a, ws);
+    if (s.epl == 16 && staged) prior_balance_kernel<T, 16, true><<<grid, block, lds, ctx->stream>>>(a, ws);
     MPC_CHECK_LAUNCH(ctx, "prior_balance");
-    prior_balance_join_kernel<<<dim3(1), dim3((a.experts + 63) / 64 * 64), 0, ctx->stream>>>(ws, blocks, a.experts, a.top_k, loss, counts, n_rows);
+    prior_balance_join_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(ws, blocks, a.experts, 1024 / a.experts, a.top_k, loss, counts, n_rows);
     MPC_CHECK_LAUNCH(ctx, "prior_balance_join");
     return MPC_OK;
 }
 
-template <typename T, int NI>
-int backward(mpc_ctx *ctx, const Row &a, const int32_t *counts, const int32_t *n_rows, const float *grad_out, void *grad, int64_t grs, int64_t ges) {
-    const int64_t b = mpc_cdiv(a.rows, PB_WAVES);
-    prior_balance_grad_kernel<T, NI><<<dim3((unsigned)(b > 4096 ? 4096 : b)), dim3(64 * PB_WAVES), 0, ctx->stream>>>(
-        a, counts, n_rows, grad_out, (T *)grad, grs, ges);
+template <typename T>
+int backward(mpc_ctx *ctx, Row a, const int32_t *counts, const int32_t *n_rows, const float *grad_out, void *grad, int64_t grs, int64_t ges) {
+    const bool staged = a.expert_stride != 1 && a.experts > 1;
+    const Shape s = shape(a, staged);
+    const dim3 grid((unsigned)(s.passes > 4096 ? 4096 : s.passes)), block(s.threads);
+    T *o = (T *)grad;
+    if (s.epl == 8 && !staged) prior_balance_grad_kernel<T, 8, false><<<grid, block, 0, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
+    if (s.epl == 8 && staged) prior_balance_grad_kernel<T, 8, true><<<grid, block, s.tile_bytes, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
+    if (s.epl == 16 && !staged) prior_balance_grad_kernel<T, 16, false><<<grid, block, 0, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
+    if (s.epl == 16 && staged) prior_balance_grad_kernel<T, 16, true><<<grid, block, s.tile_bytes, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
     MPC_CHECK_LAUNCH(ctx, "prior_balance_grad");
     return MPC_OK;
 }
@@ -197,30 +420,17 @@ int check(mpc_ctx *ctx, const void *scores, int type, int64_t rows, int experts,
     MPC_REQUIRE(ctx, rows >= 0 && rows < (1ll << 31) / top_k, "prior_balance: %lld rows", (long long)rows);
     MPC_REQUIRE(ctx, rs >= 0 && es >= 0, "prior_balance: negative stride");
     MPC_REQUIRE(ctx, scale != 0.0f && scale > -INFINITY && scale < INFINITY, "prior_balance: scale = %g", (double)scale);
-    MPC_REQUIRE(ctx, rows == 0 || scores, "prior_balance: null pointer");
+    MPC_REQUIRE(ctx, rows == 0 || (scores && (uintptr_t)scores % mpc_type_bytes(type) == 0), "prior_balance: null or misaligned pointer");
     return MPC_OK;
 }
 
 }  // namespace
 
-#define PB_BY_EXPERTS(FN, T, ...)                             \
-    do {                                                      \
-        if (experts <= 64) return FN<T, 1>(__VA_ARGS__);      \
-        if (experts <= 128) return FN<T, 2>(__VA_ARGS__);     \
-        if (experts <= 256) return FN<T, 4>(__VA_ARGS__);     \
-        if (experts <= 512) return FN<T, 8>(__VA_ARGS__);     \
-        return FN<T, 16>(__VA_ARGS__);                        \
-    } while (0)
-#define PB_DISPATCH(FN, ...)                                             \
-    do {                                                                 \
-        if (type == MPC_TYPE_F32) PB_BY_EXPERTS(FN, float, __VA_ARGS__); \
-        if (type == MPC_TYPE_F16) PB_BY_EXPERTS(FN, f16_t, __VA_ARGS__); \
-        PB_BY_EXPERTS(FN, bf16_t, __VA_ARGS__);                          \
-    } while (0)
-
 extern "C" size_t mpc_prior_balance_workspace_bytes(int64_t rows, int experts) {
     if (rows < 0 || experts <= 0 || experts > PB_MAX_EXPERTS) return 0;
-    return (size_t)blocks_for(rows) * (2 * experts + 1) * sizeof(float);
+    // as many blocks as either layout's kernel may take for these rows
+    const int64_t blocks = mpc_cdiv(rows, 2) + 1;
+    return (size_t)(blocks > PB_MAX_BLOCKS ? PB_MAX_BLOCKS : blocks) * (2 * experts + 1) * sizeof(float);
 }
 
 extern "C" int mpc_prior_balance(mpc_ctx *ctx, const void *scores, int type, int64_t rows, int experts, int64_t row_stride,
@@ -232,7 +442,9 @@ extern "C" int mpc_prior_balance(mpc_ctx *ctx, const void *scores, int type, int
     MPC_REQUIRE(ctx, workspace && loss && counts && n_rows && ((uintptr_t)workspace & 3) == 0, "prior_balance: null or misaligned pointer");
     MPC_REQUIRE(ctx, workspace_bytes >= mpc_prior_balance_workspace_bytes(rows, experts), "prior_balance: workspace of %zu bytes", workspace_bytes);
     const Row a{scores, rows, row_stride, expert_stride, experts, scale, top_k, mask};
-    PB_DISPATCH(forward, ctx, a, (float *)workspace, loss, counts, n_rows);
+    if (type == MPC_TYPE_F32) return forward<float>(ctx, a, (float *)workspace, loss, counts, n_rows);
+    if (type == MPC_TYPE_F16) return forward<f16_t>(ctx, a, (float *)workspace, loss, counts, n_rows);
+    return forward<bf16_t>(ctx, a, (float *)workspace, loss, counts, n_rows);
 }
 
 extern "C" int mpc_prior_balance_grad(mpc_ctx *ctx, const void *scores, int type, int64_t rows, int experts, int64_t row_stride,
@@ -243,8 +455,10 @@ extern "C" int mpc_prior_balance_grad(mpc_ctx *ctx, const void *scores, int type
     const int bad = check(ctx, scores, type, rows, experts, row_stride, expert_stride, scale, top_k);
     if (bad) return bad;
     if (rows == 0) return MPC_OK;
-    MPC_REQUIRE(ctx, counts && n_rows && grad, "prior_balance_grad: null pointer");
+    MPC_REQUIRE(ctx, counts && n_rows && grad && (uintptr_t)grad % mpc_type_bytes(type) == 0, "prior_balance_grad: null or misaligned pointer");
     MPC_REQUIRE(ctx, grad_row_stride >= 0 && grad_expert_stride >= 0, "prior_balance_grad: negative stride");
     const Row a{scores, rows, row_stride, expert_stride, experts, scale, top_k, mask};
-    PB_DISPATCH(backward, ctx, a, counts, n_rows, grad_out, grad, grad_row_stride, grad_expert_stride);
+    if (type == MPC_TYPE_F32) return backward<float>(ctx, a, counts, n_rows, grad_out, grad, grad_row_stride, grad_expert_stride);
+    if (type == MPC_TYPE_F16) return backward<f16_t>(ctx, a, counts, n_rows, grad_out, grad, grad_row_stride, grad_expert_stride);
+    return backward<bf16_t>(ctx, a, counts, n_rows, grad_out, grad, grad_row_stride, grad_expert_stride);
 }
