@@ -61,32 +61,56 @@ struct Or {
     __device__ __forceinline__ int operator()(int a, int b) const { return a | b; }
 };
 
-// A row's values in the order of the choice (costs negated), -inf past the last expert; all 0 if the row does not count.
+// What a lane brings of a row: its values as they lie in memory (the last expert's successors as the worst one), and whether
+// the row's mask lets it count.
 template <typename T, int EPL>
-__device__ __forceinline__ void load_values(const Row &a, const T *s, int e0, bool keep, float (&v)[EPL]) {
-    constexpr int W = 16 / sizeof(T);
+struct Raw {
+    static constexpr int W = 16 / sizeof(T);
     typedef T vec __attribute__((ext_vector_type(W)));
     typedef vec vec_any __attribute__((aligned(sizeof(T))));
+    vec t[EPL / W];
+    bool in, keep;
+
+    __device__ __forceinline__ void fetch(const Row &a, int64_t row, int e0) {
+        in = row < a.rows;
+        const int64_t at = in ? row : 0;                      // (a group without a row reads row 0 and counts nothing)
+        keep = in && (!a.mask || a.mask[at]);
+        const T *s = (const T *)a.scores + at * a.row_stride;
 #pragma unroll
-    for (int i = 0; i < EPL; i += W) {
-        if (e0 + i + W <= a.experts) {
-            const vec t = *(const vec_any *)(s + e0 + i);
+        for (int i = 0; i < EPL / W; ++i) {
+            const int e = e0 + i * W;
+            if (e + W <= a.experts) {
+                t[i] = *(const vec_any *)(s + e);
+            } else {
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[i + j] = (float)t[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < W; ++j) v[i + j] = e0 + i + j < a.experts ? (float)s[e0 + i + j] : a.scale < 0.0f ? INFINITY : -INFINITY;
+                for (int j = 0; j < W; ++j) t[i][j] = e + j < a.experts ? s[e + j] : (T)(a.scale < 0.0f ? INFINITY : -INFINITY);
+            }
         }
     }
+    // in the order of the choice (costs negated); 0 in rows that do not count
+    __device__ __forceinline__ void values(const Row &a, float (&v)[EPL]) const {
+        typedef unsigned words __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) v[j] = keep ? (a.scale < 0.0f ? -v[j] : v[j]) : 0.0f;
-}
+        for (int i = 0; i < EPL / W; ++i) {
+            words w = __builtin_bit_cast(words, t[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = keep ? w[j] : 0u;                  // (16-bit types: two values at once)
+            const vec x = __builtin_bit_cast(vec, w);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[i * W + j] = (float)x[j];
+        }
+        if (a.scale < 0.0f) {
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) v[j] = -v[j];
+        }
+    }
+};
 template <int EPL>
-__device__ __forceinline__ void load_staged(const Row &a, const float *tile_row, int e0, bool keep, float (&v)[EPL]) {
+__device__ __forceinline__ void staged_values(const Row &a, const float *tile_row, int e0, bool keep, float (&v)[EPL]) {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-        const float x = e0 + j < a.experts ? tile_row[e0 + j] : a.scale < 0.0f ? INFINITY : -INFINITY;
-        v[j] = keep ? (a.scale < 0.0f ? -x : x) : 0.0f;
+        const float x = e0 + j < a.experts ? tile_row[e0 + j] : -INFINITY;
+        v[j] = keep ? x : 0.0f;
     }
 }
 
@@ -115,17 +139,60 @@ __device__ __forceinline__ bool softmax(const Row &a, bool keep, float (&v)[EPL]
         sum += e[j];
     }
     sum = group_reduce(sum, a.group, Add());
-    inv = keep ? 1.0f / sum : 0.0f;
+    inv = keep ? __builtin_amdgcn_rcpf(sum) : 0.0f;
     return keep;
 }
 
-// Copies rows [first, first + tile_rows) to LDS, along the rows; rows behind the last become 0.
+// Copies rows [first, first + tile_rows) to LDS in the order of the choice, along the rows; rows behind the last become 0.
+// Consecutive rows (the competition's layout) come as 16 bytes of one expert's rows; with the tile's pitch of experts + 1
+// words a wave's writes fall into different banks.  Otherwise eight loads of a thread are in flight at once.
 template <typename T>
 __device__ __forceinline__ void stage(const Row &a, int64_t first, float *tile) {
-    const int pitch = a.experts + 1;
-    for (int i = threadIdx.x; i < a.experts << a.tile_log2; i += blockDim.x) {
-        const int r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
-        tile[r * pitch + e] = first + r < a.rows ? (float)((const T *)a.scores)[(first + r) * a.row_stride + e * a.expert_stride] : 0.0f;
+    constexpr int U = 8, W = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(W)));
+    typedef vec vec_any __attribute__((aligned(sizeof(T))));
+    const int pitch = a.experts + 1, all = a.experts << a.tile_log2, step = blockDim.x;
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+    const T *s = (const T *)a.scores + first * a.row_stride;
+    const int64_t left = a.rows - first;
+    if (a.row_stride == 1) {
+        constexpr int V = 2;                                  // (tile_rows is a multiple of W)
+        for (int base = threadIdx.x * W; base < all; base += V * step * W) {
+            vec x[V];
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                const int i = base + u * step * W, r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
+                if (i < all && r + W <= left) {
+                    x[u] = *(const vec_any *)(s + r + e * a.expert_stride);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) x[u][j] = i < all && r + j < left ? s[r + j + e * a.expert_stride] : (T)0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                const int i = base + u * step * W, r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
+                if (i < all) {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) tile[(r + j) * pitch + e] = (float)x[u][j] * sign;
+                }
+            }
+        }
+        return;
+    }
+    for (int base = threadIdx.x; base < all; base += U * step) {
+        T x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = base + u * step, r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
+            x[u] = (T)0.0f;
+            if (i < all && r < left) x[u] = s[r * a.row_stride + e * a.expert_stride];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = base + u * step;
+            if (i < all) tile[(i & (a.tile_rows - 1)) * pitch + (i >> a.tile_log2)] = (float)x[u] * sign;
+        }
     }
 }
 
@@ -145,16 +212,11 @@ __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_kernel(Row a, fl
 #pragma unroll
     for (int j = 0; j < EPL; ++j) acc[j] = 0.0f;
 
-    auto one = [&](int64_t row, const float *tile_row) {
-        const bool in = row < a.rows;
-        const int64_t at = in ? row : 0;                      // (a group without a row reads row 0 and counts nothing)
-        bool keep = in && (!a.mask || a.mask[at]);
-        float v[EPL], e[EPL], top, inv;
-        if constexpr (STAGED) load_staged<EPL>(a, tile_row, e0, keep, v);
-        else load_values<T, EPL>(a, (const T *)a.scores + at * a.row_stride, e0, keep, v);
+    auto one = [&](bool keep, float (&v)[EPL]) {
+        float e[EPL], top, inv;
         keep = softmax<EPL>(a, keep, v, e, top, inv);
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) acc[j] = fmaf(keep ? e[j] : 0.0f, inv, acc[j]);
+        for (int j = 0; j < EPL; ++j) acc[j] = fmaf(e[j], inv, acc[j]);          // (rows that do not count: inv = 0, e finite)
         n += (int)__popcll(__ballot(keep && e0 == 0));
         for (int k = 0; k < a.top_k; ++k) {
             float best = top;
@@ -182,14 +244,26 @@ __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_kernel(Row a, fl
             __syncthreads();
             for (int r = wave * per_wave; r < a.tile_rows; r += per_block) {
                 const int mine = r + (lane >> a.group_log2);  // (tile_rows may be less than a wave's rows)
-                const bool in = mine < a.tile_rows;
-                one(in ? first + mine : a.rows, tile + (in ? mine : 0) * (a.experts + 1));
+                const bool in = mine < a.tile_rows && first + mine < a.rows;
+                float v[EPL];
+                const bool keep = in && (!a.mask || a.mask[first + mine]);
+                staged_values<EPL>(a, tile + (in ? mine : 0) * (a.experts + 1), e0, keep, v);
+                one(keep, v);
             }
         }
         __syncthreads();
     } else {
-        for (int64_t first = (int64_t)blockIdx.x * per_block + wave * per_wave; first < a.rows; first += (int64_t)gridDim.x * per_block)
-            one(first + (lane >> a.group_log2), nullptr);
+        const int64_t step = (int64_t)gridDim.x * per_block;
+        int64_t first = (int64_t)blockIdx.x * per_block + wave * per_wave;
+        Raw<T, EPL> now, next;
+        if (first < a.rows) now.fetch(a, first + (lane >> a.group_log2), e0);
+        for (; first < a.rows; first += step) {               // the next rows are on their way while these are worked on
+            if (first + step < a.rows) next.fetch(a, first + step + (lane >> a.group_log2), e0);
+            float v[EPL];
+            now.values(a, v);
+            one(now.keep, v);
+            now = next;
+        }
     }
 
     // the groups of a wave, then the waves of the block
@@ -279,17 +353,13 @@ __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_grad_kernel(Row 
         f[j] = e0 + j < a.experts && n > 0 ? (float)((double)counts[e0 + j] / ((double)a.top_k * n) - 1.0 / a.experts) : 0.0f;
     const float g = n > 0 ? (float)((double)(grad_out ? *grad_out : 1.0f) * a.scale * a.experts / n) : 0.0f;
 
-    auto one = [&](int64_t row, bool in, float *tile_row) {
-        const int64_t at = in ? row : 0;
-        bool keep = in && (!a.mask || a.mask[at]);
-        float v[EPL], e[EPL], top, inv;
-        if constexpr (STAGED) load_staged<EPL>(a, tile_row, e0, keep, v);
-        else load_values<T, EPL>(a, (const T *)a.scores + at * a.row_stride, e0, keep, v);
+    auto one = [&](int64_t row, bool in, bool keep, float (&v)[EPL], float *tile_row) {
+        float e[EPL], top, inv;
         keep = softmax<EPL>(a, keep, v, e, top, inv);
         float d = 0.0f;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
-            e[j] = keep ? e[j] * inv : 0.0f;
+            e[j] *= inv;                                      // (rows that do not count: inv = 0, e finite)
             d = fmaf(e[j], f[j], d);
         }
         d = group_reduce(d, a.group, Add());
@@ -332,19 +402,47 @@ __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_grad_kernel(Row 
             __syncthreads();
             for (int r = wave * per_wave; r < a.tile_rows; r += per_block) {
                 const int mine = r + (lane >> a.group_log2);
-                const bool in = mine < a.tile_rows;
-                one(first + mine, in && first + mine < a.rows, tile + (in ? mine : 0) * pitch);
+                const bool in = mine < a.tile_rows && first + mine < a.rows;
+                float *tile_row = tile + (in ? mine : 0) * pitch;
+                float v[EPL];
+                const bool keep = in && (!a.mask || a.mask[first + mine]);
+                staged_values<EPL>(a, tile_row, e0, keep, v);
+                one(first + mine, in, keep, v, tile_row);
             }
             __syncthreads();
-            for (int i = tid; i < a.experts << a.tile_log2; i += blockDim.x) {
-                const int r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
-                if (first + r < a.rows) grad[(first + r) * grs + e * ges] = (T)tile[r * pitch + e];
+            if (grs == 1) {
+                for (int i = tid * W; i < a.experts << a.tile_log2; i += blockDim.x * W) {
+                    const int r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
+                    T *o = grad + first + r + e * ges;
+                    vec t;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) t[j] = (T)tile[(r + j) * pitch + e];
+                    if (first + r + W <= a.rows) {
+                        *(vec_any *)o = t;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < W; ++j)
+                            if (first + r + j < a.rows) o[j] = t[j];
+                    }
+                }
+            } else {
+                for (int i = tid; i < a.experts << a.tile_log2; i += blockDim.x) {
+                    const int r = i & (a.tile_rows - 1), e = i >> a.tile_log2;
+                    if (first + r < a.rows) grad[(first + r) * grs + e * ges] = (T)tile[r * pitch + e];
+                }
             }
         }
     } else {
-        for (int64_t first = (int64_t)blockIdx.x * per_block + wave * per_wave; first < a.rows; first += (int64_t)gridDim.x * per_block) {
-            const int64_t row = first + (lane >> a.group_log2);
-            one(row, row < a.rows, nullptr);
+        const int64_t step = (int64_t)gridDim.x * per_block;
+        int64_t first = (int64_t)blockIdx.x * per_block + wave * per_wave;
+        Raw<T, EPL> now, next;
+        if (first < a.rows) now.fetch(a, first + (lane >> a.group_log2), e0);
+        for (; first < a.rows; first += step) {
+            if (first + step < a.rows) next.fetch(a, first + step + (lane >> a.group_log2), e0);
+            float v[EPL];
+            now.values(a, v);
+            one(first + (lane >> a.group_log2), now.in, now.keep, v, nullptr);
+            now = next;
         }
     }
 }
@@ -366,6 +464,7 @@ Shape shape(Row &a, bool staged) {
     if (staged) {
         int r = few ? 16 : 64;
         while (r > 8 && r * (a.experts + 1) > 12288) r /= 2;
+        while (!few && r * a.group < PB_MAX_THREADS && 2 * r * (a.experts + 1) <= 12288) r *= 2;    // (few experts: rows enough for the block)
         a.tile_rows = r;
         a.tile_log2 = __builtin_ctz(r);
         const int t = r * a.group;
@@ -403,7 +502,7 @@ template <typename T>
 int backward(mpc_ctx *ctx, Row a, const int32_t *counts, const int32_t *n_rows, const float *grad_out, void *grad, int64_t grs, int64_t ges) {
     const bool staged = a.expert_stride != 1 && a.experts > 1;
     const Shape s = shape(a, staged);
-    const dim3 grid((unsigned)(s.passes > 4096 ? 4096 : s.passes)), block(s.threads);
+    const dim3 grid((unsigned)(s.passes > 1024 ? 1024 : s.passes)), block(s.threads);
     T *o = (T *)grad;
     if (s.epl == 8 && !staged) prior_balance_grad_kernel<T, 8, false><<<grid, block, 0, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
     if (s.epl == 8 && staged) prior_balance_grad_kernel<T, 8, true><<<grid, block, s.tile_bytes, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
