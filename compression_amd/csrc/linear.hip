@@ -8,8 +8,11 @@
 // outputs of one row and stores them as 16-byte pieces.
 #include "row_ops.h"
 
+#include <type_traits>
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x8 __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4_any __attribute__((aligned(1)));          // a 16-byte access at any address
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -57,64 +60,95 @@ __device__ __forceinline__ void activate(float (&v)[V], int act) {
     }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void finish(const LinearArgs &a, int64_t m, int64_t n, float (&v)[V]) {
-    constexpr int PER = 16 / sizeof(T);
+// The rows of a lane: row0 + 16 m, columns n .. n + V - 1; take(m, v) gives the sums.  One rolled loop (the sums have fixed
+// registers, so take is a switch over copies): unrolled it would be tens of KB of code.  The next row's residual is on its way while
+// a row is worked on.
+template <typename T, int MF, int V, typename Take>
+__device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, int64_t n, Take take) {
+    constexpr int PER = 16 / sizeof(T), P = V / PER;
     typedef T vec_t __attribute__((ext_vector_type(PER)));
-    const bool whole = n + V <= a.N;
-    if (a.res) {
-        const T *r = (const T *)(a.res + m * a.rs) + n;
-        if (whole && a.vec_res) {
-#pragma unroll
-            for (int i = 0; i < V; i += PER) {
-                const vec_t t = *(const vec_t *)(r + i);
-#pragma unroll
-                for (int j = 0; j < PER; ++j) v[i + j] += (float)t[j];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (n + i < a.N) v[i] += (float)r[i];
-        }
-    }
-    T *o = (T *)(a.out + m * a.os) + n;
-    if (whole && a.vec_out) {
-#pragma unroll
-        for (int i = 0; i < V; i += PER) {
-            vec_t t;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) t[j] = (T)v[i + j];
-            *(vec_t *)(o + i) = t;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (n + i < a.N) o[i] = (T)v[i];
-    }
-}
-
-template <int V>
-__device__ __forceinline__ void column_terms(const LinearArgs &a, int64_t n, float (&b)[V], float (&s)[V]) {
+    const bool whole = n + V <= a.N, vec_out = whole && a.vec_out, vec_res = a.res && whole && a.vec_res;
+    float b[V], s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         b[i] = a.bias && n + i < a.N ? a.bias[n + i] : 0.0f;
         s[i] = a.sw && n + i < a.N ? a.sw[n + i] : 1.0f;
     }
+    vec_t next[P];
+    auto fetch = [&](int64_t row) {
+        const T *r = (const T *)(a.res + row * a.rs) + n;
+#pragma unroll
+        for (int i = 0; i < P; ++i) next[i] = *(const vec_t *)(r + i * PER);
+    };
+    if (vec_res && row0 < a.M) fetch(row0);
+#pragma unroll 1
+    for (int m = 0; m < MF; ++m) {
+        const int64_t row = row0 + 16 * m;
+        float v[V];
+        take(m, v);
+        if (row >= a.M) break;
+        vec_t res[P];
+        if (vec_res) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) res[i] = next[i];
+            if (m + 1 < MF && row + 16 < a.M) fetch(row + 16);
+        }
+        if (a.sx) {
+            const float sx = a.sx[row];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] *= sx * s[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] += b[i];
+        activate<V>(v, a.act);
+        if (vec_res) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] += (float)res[i / PER][i % PER];
+        } else if (a.res) {
+            const T *r = (const T *)(a.res + row * a.rs) + n;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (n + i < a.N) v[i] += (float)r[i];
+        }
+        T *o = (T *)(a.out + row * a.os) + n;
+        if (vec_out) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                vec_t t;
+#pragma unroll
+                for (int q = 0; q < PER; ++q) t[q] = (T)v[i * PER + q];
+                *(vec_t *)(o + i * PER) = t;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (n + i < a.N) o[i] = (T)v[i];
+        }
+    }
 }
 
-template <int V>
-__device__ __forceinline__ void epilogue(const LinearArgs &a, int64_t m, int64_t n, float (&v)[V], const float (&b)[V], const float (&s)[V]) {
-    const float sx = a.sx ? a.sx[m] : 1.0f;
-    if (a.sx) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] *= sx * s[i];
+template <int MF, int V, typename Take>
+__device__ __forceinline__ void epilogue(const LinearArgs &a, int64_t row0, int64_t n, Take take) {
+    if (n >= a.N) return;
+    if (a.out_type == MPC_TYPE_F32) finish_rows<float, MF, V>(a, row0, n, take);
+    else if (a.out_type == MPC_TYPE_F16) finish_rows<f16_t, MF, V>(a, row0, n, take);
+    else finish_rows<bf16_t, MF, V>(a, row0, n, take);
+}
+
+// sums of x tile m as the V consecutive outputs of a lane's row
+template <int MF, int NF, int M = 0>
+__device__ __forceinline__ void take_tile(const f32x4 (&acc)[NF][MF], int m, float (&v)[4 * NF]) {
+    if constexpr (M + 1 < MF) {
+        if (m != M) return take_tile<MF, NF, M + 1>(acc, m, v);
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] += b[i];
-    activate<V>(v, a.act);
-    if (a.out_type == MPC_TYPE_F32) finish<float, V>(a, m, n, v);
-    else if (a.out_type == MPC_TYPE_F16) finish<f16_t, V>(a, m, n, v);
-    else finish<bf16_t, V>(a, m, n, v);
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float t = acc[f][M][r];
+            asm("" : "+v"(t));                  // (else the copies are merged into one through a pointer, and the sums go to memory for it)
+            v[4 * f + r] = t;
+        }
 }
 
 // ---- operands ---------------------------------------------------------------------------------------------------------
@@ -268,21 +302,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void linear_tile_kernel
         __syncthreads();
     }
 
-    const int64_t n = n0 + wn + g * V;
-    if (n >= a.N) return;
-    float b[V], s[V];
-    column_terms<V>(a, n, b, s);
-#pragma unroll
-    for (int m = 0; m < MF; ++m) {
-        const int64_t row = m0 + wm + m * 16 + j;
-        if (row >= a.M) continue;
-        float v[V];
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[4 * f + r] = acc[f][m][r];
-        epilogue<V>(a, row, n, v, b, s);
-    }
+    epilogue<MF, V>(a, m0 + wm + j, n0 + wn + g * V, [&](int m, float (&v)[V]) { take_tile<MF, NF>(acc, m, v); });
 }
 
 template <int TYPE, int BM, int BN, int WM, int WN>
@@ -304,8 +324,200 @@ int launch_tiles(mpc_ctx *ctx, LinearArgs a) {
     return MPC_OK;
 }
 
+// ---- large products: 256 x 256 tiles, one workgroup per CU -------------------------------------------------------------------
+// Four waves, each 128 x 128 outputs in 256 accumulator registers: a wave then reads 32 KB of LDS per k-tile for 2048 cycles
+// of matrix instructions (the four of a CU 64 bytes a cycle; waves of 64 x 64 would need all 128 that LDS delivers).  With one
+// wave per SIMD nothing else hides its latencies, so they are hidden in the wave itself: a k-tile is four quadrants of
+// 64 x 64, and while one multiplies, the operands of the next come from LDS, the pieces of the next k-tile go from
+// registers to the other LDS buffer and those of the one after leave for memory.  The last quadrant of a tile shares no
+// operand with the first of the next, so the order of the w halves alternates from tile to tile.
+constexpr int BIG = 256;
+
+__device__ __forceinline__ void lds_barrier() {               // LDS accesses done, then the barrier; memory loads stay in flight
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Tile of workgroup b: each XCD (workgroups go to the 8 in turn) gets a contiguous run of the tiles, in groups of 8 tile
+// rows with the rows innermost, so that the tiles an XCD works on at a time share operands in its L2.
+__device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int &tm, int &tn) {
+    const int total = tiles_m * tiles_n, xcd = b & 7, per = total >> 3, rest = total & 7;
+    const int i = xcd * per + (xcd < rest ? xcd : rest) + (b >> 3);
+    const int group = 8 * tiles_n, first = i / group * 8, rows = tiles_m - first < 8 ? tiles_m - first : 8, in = i % group;
+    tm = first + in % rows;
+    tn = in / rows;
+}
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+
+// c += a b with c in accumulation registers, in place.  All 256 of them hold sums here; through the builtin the compiler moves
+// sums from register to register (a result need not go where its input was), with none left to move them through: twice as
+// many moves as products, and spills.  Operands come from LDS or memory reads, which the compiler waits for; two
+// instructions on the same sums are at least 16 apart, and the kernel waits before it reads them.
+template <int TYPE>
+__device__ __forceinline__ void mma_in_place(u32x4 a, u32x4 b, f32x4 &c) {
+    if constexpr (TYPE == MPC_TYPE_F16) asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+template <int TYPE>
+__device__ __forceinline__ void mma_in_place(u32x4 a0, u32x4 a1, u32x4 b0, u32x4 b1, f32x4 &c) {
+    const u32x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+    asm("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));       // (both formats default to e4m3, no block scales)
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
+    constexpr int V = 32;                                     // consecutive outputs of a lane
+    extern __shared__ u32x4 lds[];                            // 2 x [256 rows of x, 256 of w][8 pieces]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int j = lane & 15, g = lane >> 4;
+    const int wm = (wave & 1) * 128, wn = (wave >> 1) * 128;
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    const int64_t m0 = (int64_t)tm * BIG, n0 = (int64_t)tn * BIG;
+    const int rows_x = (int)(a.M - m0 < BIG ? a.M - m0 : BIG), rows_w = (int)(a.N - n0 < BIG ? a.N - n0 : BIG);
+
+    // Pieces come by buffer loads with the tile's own rows as bounds: a row past the last, or a piece past K (a multiple of 16
+    // bytes here), gets an offset past the end, and such a load gives zeros.
+    constexpr unsigned NO_ROW = 0x80000000u, NO_K = 0x40000000u;   // (the tile ends below 2^30: the host checks)
+    const rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.x + m0 * a.xs), 0, (int)((rows_x - 1) * a.xs + a.K), 0x00020000);
+    const rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + n0 * a.ws), 0, (int)((rows_w - 1) * a.ws + a.K), 0x00020000);
+    const int p = tid & 7, r0 = tid >> 3;
+    unsigned xo[8], wo[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = r0 + 32 * i;
+        xo[i] = r < rows_x ? (unsigned)(r * a.xs) + p * 16 : NO_ROW;
+        wo[i] = r < rows_w ? (unsigned)(r * a.ws) + p * 16 : NO_ROW;
+    }
+    u32x4 xg[8], wg[8];
+    const int K = (int)a.K;
+    auto k_offset = [&](int k) { return k + p * 16 < K ? (unsigned)k : NO_K; };
+    auto fetch_x = [&](int i, unsigned ko) { xg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, xo[i] + ko, 0, 0)); };
+    auto fetch_w = [&](int i, unsigned ko) { wg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, wo[i] + ko, 0, 0)); };
+    // LDS slots, as in the kernel above: piece p of row r at p ^ key(r); rows of w are read interleaved in runs of V, so its
+    // key takes bit 5 of the row.  [x buffer 0][x buffer 1][w buffer 0][w buffer 1], each 256 rows of 8 pieces.
+    u32x4 *const xdst = lds + r0 * 8 + (p ^ (r0 & 7));
+    u32x4 *const wdst0 = lds + 2 * BIG * 8 + r0 * 8 + (p ^ (r0 & 3)), *const wdst1 = lds + 2 * BIG * 8 + r0 * 8 + (p ^ ((r0 & 3) | 4));
+    auto stash_x = [&](int i, int buf) { xdst[buf * (BIG * 8) + i * 256] = xg[i]; };
+    auto stash_w = [&](int i, int buf) { (i & 1 ? wdst1 : wdst0)[buf * (BIG * 8) + i * 256] = wg[i]; };
+    struct Half {                                             // 64 rows: 4 tiles x 2 pieces
+        u32x4 v[4][2];
+    };
+    const u32x4 *const xsrc[2] = {lds + (wm + j) * 8 + (g ^ (j & 7)), lds + (wm + j) * 8 + ((4 + g) ^ (j & 7))};
+    const int wrow = wn + (j >> 2) * V + (j & 3), wkey = (j & 3) | (j >> 2 & 1) << 2;
+    const u32x4 *const wsrc[2] = {lds + 2 * BIG * 8 + wrow * 8 + (g ^ wkey), lds + 2 * BIG * 8 + wrow * 8 + ((4 + g) ^ wkey)};
+    auto read_x = [&](Half &h, int i, int buf, int half) { h.v[i & 3][i >> 2] = xsrc[i >> 2][buf * (BIG * 8) + (half * 4 + (i & 3)) * 128]; };
+    auto read_w = [&](Half &h, int i, int buf, int half) { h.v[i & 3][i >> 2] = wsrc[i >> 2][buf * (BIG * 8) + (half * 4 + (i & 3)) * 32]; };
+
+    f32x4 acc[8][8];                                          // [w tile][x tile]
+#pragma unroll
+    for (int f = 0; f < 8; ++f)
+#pragma unroll
+        for (int m = 0; m < 8; ++m) acc[f][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // One quadrant in eight groups of matrix instructions; beside(i) issues what goes with group i.
+    auto multiply = [&](const Half &w, const Half &x, auto wh, auto xh, auto beside) {
+        constexpr int F = decltype(wh)::value * 4, M = decltype(xh)::value * 4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            beside(i);
+            if constexpr (TYPE == MPC_TYPE_E4M3) {
+#pragma unroll
+                for (int m = 2 * (i & 1); m < 2 * (i & 1) + 2; ++m)
+                    mma_in_place<TYPE>(w.v[i >> 1][0], w.v[i >> 1][1], x.v[m][0], x.v[m][1], acc[F + (i >> 1)][M + m]);
+            } else {
+#pragma unroll
+                for (int m = 0; m < 4; ++m) mma_in_place<TYPE>(w.v[i & 3][i >> 2], x.v[m][i >> 2], acc[F + (i & 3)][M + m]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    using Lo = std::integral_constant<int, 0>;
+    using Hi = std::integral_constant<int, 1>;
+    Half x0, x1, w0, w1;
+    // One k-tile from buffer `buf`; x0 and the first w half (wa) are in registers, the pieces of the next tile in xg, wg or on
+    // their way.  k2: where the tile after the next begins (past the end: zeros are fetched, and never read).
+    auto tile = [&](int buf, int k2, Half &wa, Half &wb, auto ha, auto hb) {
+        constexpr int WB = decltype(hb)::value;
+        const unsigned ko = k_offset(k2);
+        multiply(wa, x0, ha, Lo{}, [&](int i) {
+            if (i < 4) read_w(wb, 2 * i, buf, WB), read_w(wb, 2 * i + 1, buf, WB);
+        });
+        multiply(wb, x0, hb, Lo{}, [&](int i) {
+            if (i < 4) read_x(x1, 2 * i, buf, 1), read_x(x1, 2 * i + 1, buf, 1);
+            else stash_x(2 * i - 8, buf ^ 1), stash_x(2 * i - 7, buf ^ 1);
+        });
+        multiply(wb, x1, hb, Hi{}, [&](int i) {
+            if (i < 4) stash_w(2 * i, buf ^ 1), stash_w(2 * i + 1, buf ^ 1);
+            else fetch_x(2 * i - 8, ko), fetch_x(2 * i - 7, ko);
+        });
+        lds_barrier();
+        multiply(wa, x1, ha, Hi{}, [&](int i) {
+            if (i < 4) {
+                read_x(x0, 2 * i, buf ^ 1, 0), read_x(x0, 2 * i + 1, buf ^ 1, 0);
+                read_w(wb, 2 * i, buf ^ 1, WB), read_w(wb, 2 * i + 1, buf ^ 1, WB);
+            } else {
+                fetch_w(2 * i - 8, ko), fetch_w(2 * i - 7, ko);
+            }
+        });
+    };
+    const unsigned k0 = k_offset(0), k1 = k_offset(KT);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fetch_x(i, k0), fetch_w(i, k0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) stash_x(i, 0), stash_w(i, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fetch_x(i, k1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fetch_w(i, k1);
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) read_x(x0, i, 0, 0), read_w(w0, i, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 7" ::: "memory");                     // (the zeros just written to the accumulators: two states before their first use)
+    __builtin_amdgcn_sched_barrier(0);
+    // Two tiles a turn, an odd last one beside one of zeros: its operands past K are all zero, so it adds nothing.
+    int k = 0;
+    do {
+        tile(0, k + 2 * KT, w0, w1, Lo{}, Hi{});
+        tile(1, k + 3 * KT, w1, w0, Hi{}, Lo{});
+        k += 2 * KT;
+    } while (k < K);
+    // The compiler does not see that the last instructions above write accumulators: their results are complete behind this.
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+
+    epilogue<8, V>(a, m0 + wm + j, n0 + wn + g * V, [&](int m, float (&v)[V]) { take_tile<8, 8>(acc, m, v); });
+}
+
+template <int TYPE>
+int launch_big(mpc_ctx *ctx, LinearArgs a) {
+    constexpr size_t lds = 2 * 2 * BIG * KT;
+    auto kern = linear_big_kernel<TYPE>;
+    static bool attr_set[MPC_MAX_DEVICES] = {};
+    bool &attr_done = attr_set[ctx->device];
+    if (!attr_done) {
+        MPC_HIP(ctx, hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        attr_done = true;
+    }
+    a.tiles_m = (int)mpc_cdiv(a.M, BIG);
+    a.tiles_n = (int)mpc_cdiv(a.N, BIG);
+    kern<<<dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), lds, ctx->stream>>>(a);
+    MPC_CHECK_LAUNCH(ctx, "linear_big");
+    return MPC_OK;
+}
+
+// 16-byte pieces everywhere, and offsets inside a tile that 30 bits hold
+bool big_possible(const LinearArgs &a) {
+    return ((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.xs | (uintptr_t)a.ws | (uintptr_t)a.K) % 16 == 0 &&
+           BIG * a.xs + a.K < (1ll << 30) && BIG * a.ws + a.K < (1ll << 30) && mpc_cdiv(a.M, BIG) * mpc_cdiv(a.N, BIG) < (1ll << 31);
+}
+
 template <int TYPE>
 int launch(mpc_ctx *ctx, const LinearArgs &a) {
+    if (big_possible(a) && mpc_cdiv(a.M, BIG) * mpc_cdiv(a.N, BIG) >= 256) return launch_big<TYPE>(ctx, a);
     return launch_tiles<TYPE, 128, 128, 64, 64>(ctx, a);
 }
 

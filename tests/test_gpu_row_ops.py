@@ -197,7 +197,8 @@ def test_linear(dtype, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
-@pytest.mark.parametrize("M,N,K", SIZES + [(700, 900, 2000), (3, 4096, 4096), (5000, 260, 1030)])
+@pytest.mark.parametrize("M,N,K", SIZES + [(700, 900, 2000), (3, 4096, 4096), (5000, 260, 1030), (4200, 4104, 512), (4097, 4160, 16), (66000, 250, 80),
+                                           (4352, 4096, 144), (200, 70000, 208), (5000, 4000, 1152)])
 def test_linear_whole_numbers_exactly(dtype, M, N, K):
     """Small whole operands: every product and sum is a whole number below 2^24, exact in fp32 and on the 8-bit
     instructions' grid, so one value of k too many, too few or in the wrong place shows."""
@@ -214,7 +215,7 @@ def test_linear_whole_numbers_exactly(dtype, M, N, K):
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("M,N,K", [(2100, 2050, 520), (4096, 1024, 256), (8200, 256, 1024), (3000, 4100, 136), (9, 4096, 4096), (300, 4096, 2048),
-                                   (36864, 64, 256), (2048, 2048, 2048), (5000, 1030, 1040)])
+                                   (36864, 64, 256), (2048, 2048, 2048), (5000, 1030, 1040), (4200, 4104, 512), (8192, 2048, 272)])
 def test_linear_large(dtype, M, N, K):
     from compression_amd import ops
     x, w, sx, sw = operands(M + N + K, M, N, K, dtype)
