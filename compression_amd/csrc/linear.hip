@@ -3,9 +3,9 @@
 // Both operands lie with k innermost, which is how the matrix instructions want them: a lane of a 16x16 tile holds 16
 // (16-bit operands: 8 values; e4m3: 16, two such pieces) consecutive bytes of one row.  A k-tile is 128 bytes of every
 // row, 64 values of 16 bits or 128 of 8, so both widths move the same bytes and issue the same matrix cycles per tile.
-// w is the instruction's first operand: a lane then holds four consecutive n of one m.  Which row of w a lane
-// brings is free, so the NF tiles side by side take rows interleaved in fours: a lane ends up with 4 NF consecutive
-// outputs of one row and stores them as 16-byte pieces.
+// w is the instruction's first operand: a lane then holds four consecutive n of one m.  Which row of w a lane brings is
+// free, so two tiles take the rows of 32 columns interleaved in fours: a lane ends up with runs of 8 consecutive outputs of
+// one row, 16 bytes of a 16-bit type, and the four lanes of a row with 32 consecutive ones.
 #include "row_ops.h"
 
 #include <type_traits>
@@ -60,25 +60,27 @@ __device__ __forceinline__ void activate(float (&v)[V], int act) {
     }
 }
 
-// The rows of a lane: row0 + 16 m, columns n .. n + V - 1; take(m, v) gives the sums.  One rolled loop (the sums have fixed
+// The rows of a lane: row0 + 16 m; its V columns are V / 8 runs of 8, n + 32 t .. n + 32 t + 7: the four lanes of a row then
+// write 64 consecutive bytes at a time.  take(m, v) gives the sums.  One rolled loop (the sums have fixed
 // registers, so take is a switch over copies): unrolled it would be tens of KB of code.  The next row's residual is on its way while
 // a row is worked on.
 template <typename T, int MF, int V, typename Take>
 __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, int64_t n, Take take) {
     constexpr int PER = 16 / sizeof(T), P = V / PER;
     typedef T vec_t __attribute__((ext_vector_type(PER)));
-    const bool whole = n + V <= a.N, vec_out = whole && a.vec_out, vec_res = a.res && whole && a.vec_res;
+    auto col = [&](int i) { return n + (i & 7) + 32 * (i >> 3); };          // column of value i
+    const bool whole = col(V - 1) < a.N, vec_out = whole && a.vec_out, vec_res = a.res && whole && a.vec_res;
     float b[V], s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        b[i] = a.bias && n + i < a.N ? a.bias[n + i] : 0.0f;
-        s[i] = a.sw && n + i < a.N ? a.sw[n + i] : 1.0f;
+        b[i] = a.bias && col(i) < a.N ? a.bias[col(i)] : 0.0f;
+        s[i] = a.sw && col(i) < a.N ? a.sw[col(i)] : 1.0f;
     }
     vec_t next[P];
     auto fetch = [&](int64_t row) {
-        const T *r = (const T *)(a.res + row * a.rs) + n;
+        const T *r = (const T *)(a.res + row * a.rs);
 #pragma unroll
-        for (int i = 0; i < P; ++i) next[i] = *(const vec_t *)(r + i * PER);
+        for (int i = 0; i < P; ++i) next[i] = *(const vec_t *)(r + col(i * PER));
     };
     if (vec_res && row0 < a.M) fetch(row0);
 #pragma unroll 1
@@ -105,24 +107,24 @@ __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, i
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] += (float)res[i / PER][i % PER];
         } else if (a.res) {
-            const T *r = (const T *)(a.res + row * a.rs) + n;
+            const T *r = (const T *)(a.res + row * a.rs);
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (n + i < a.N) v[i] += (float)r[i];
+                if (col(i) < a.N) v[i] += (float)r[col(i)];
         }
-        T *o = (T *)(a.out + row * a.os) + n;
+        T *o = (T *)(a.out + row * a.os);
         if (vec_out) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 vec_t t;
 #pragma unroll
                 for (int q = 0; q < PER; ++q) t[q] = (T)v[i * PER + q];
-                *(vec_t *)(o + i * PER) = t;
+                *(vec_t *)(o + col(i * PER)) = t;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (n + i < a.N) o[i] = (T)v[i];
+                if (col(i) < a.N) o[col(i)] = (T)v[i];
         }
     }
 }
@@ -135,7 +137,7 @@ __device__ __forceinline__ void epilogue(const LinearArgs &a, int64_t row0, int6
     else finish_rows<bf16_t, MF, V>(a, row0, n, take);
 }
 
-// sums of x tile m as the V consecutive outputs of a lane's row
+// sums of x tile m as the V outputs of a lane's row
 template <int MF, int NF, int M = 0>
 __device__ __forceinline__ void take_tile(const f32x4 (&acc)[NF][MF], int m, float (&v)[4 * NF]) {
     if constexpr (M + 1 < MF) {
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void linear_tile_kernel
 
     // Piece p of row r lies at slot p ^ key(r): the 16 rows that one instruction reads at the same p then spread over the banks.
     auto xkey = [](int r) { return r & 7; };
-    auto wkey = [](int r) { return (r & 3) | (r / V & 1) << 2; };
+    auto wkey = [](int r) { return (r & 3) | (r >> 3 & 1) << 2; };
 
     const int p = tid & 7;
     const char *xp[XP], *wp[WP];
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void linear_tile_kernel
             return x[r * 8 + (q ^ xkey(r))];
         };
         auto wfrag = [&](int f, int q) {
-            const int r = wn + (j >> 2) * V + f * 4 + (j & 3);
+            const int r = wn + (f >> 1) * 32 + (j >> 2) * 8 + (f & 1) * 4 + (j & 3);
             return w[r * 8 + (q ^ wkey(r))];
         };
         if constexpr (TYPE == MPC_TYPE_E4M3) {
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void linear_tile_kernel
         __syncthreads();
     }
 
-    epilogue<MF, V>(a, m0 + wm + j, n0 + wn + g * V, [&](int m, float (&v)[V]) { take_tile<MF, NF>(acc, m, v); });
+    epilogue<MF, V>(a, m0 + wm + j, n0 + wn + g * 8, [&](int m, float (&v)[V]) { take_tile<MF, NF>(acc, m, v); });
 }
 
 template <int TYPE, int BM, int BN, int WM, int WN>
@@ -396,20 +398,25 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     auto k_offset = [&](int k) { return k + p * 16 < K ? (unsigned)k : NO_K; };
     auto fetch_x = [&](int i, unsigned ko) { xg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, xo[i] + ko, 0, 0)); };
     auto fetch_w = [&](int i, unsigned ko) { wg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, wo[i] + ko, 0, 0)); };
-    // LDS slots, as in the kernel above: piece p of row r at p ^ key(r); rows of w are read interleaved in runs of V, so its
-    // key takes bit 5 of the row.  [x buffer 0][x buffer 1][w buffer 0][w buffer 1], each 256 rows of 8 pieces.
+    // LDS slots, as in the kernel above: piece p of row r at p ^ key(r); rows of w are read interleaved, so its
+    // key takes bit 3 of the row.  [x buffer 0][x buffer 1][w buffer 0][w buffer 1], each 256 rows of 8 pieces.
     u32x4 *const xdst = lds + r0 * 8 + (p ^ (r0 & 7));
-    u32x4 *const wdst0 = lds + 2 * BIG * 8 + r0 * 8 + (p ^ (r0 & 3)), *const wdst1 = lds + 2 * BIG * 8 + r0 * 8 + (p ^ ((r0 & 3) | 4));
+    u32x4 *const wdst = lds + 2 * BIG * 8 + r0 * 8 + (p ^ ((r0 & 3) | (r0 >> 3 & 1) << 2));
     auto stash_x = [&](int i, int buf) { xdst[buf * (BIG * 8) + i * 256] = xg[i]; };
-    auto stash_w = [&](int i, int buf) { (i & 1 ? wdst1 : wdst0)[buf * (BIG * 8) + i * 256] = wg[i]; };
+    auto stash_w = [&](int i, int buf) { wdst[buf * (BIG * 8) + i * 256] = wg[i]; };
+    // Piece n of 16 goes to LDS and the one of the tile after leaves for its registers at once: it has a whole k-tile's time to arrive.
+    auto move = [&](int n, int buf, unsigned ko) {
+        if (n < 8) stash_x(n, buf), fetch_x(n, ko);
+        else stash_w(n - 8, buf), fetch_w(n - 8, ko);
+    };
     struct Half {                                             // 64 rows: 4 tiles x 2 pieces
         u32x4 v[4][2];
     };
     const u32x4 *const xsrc[2] = {lds + (wm + j) * 8 + (g ^ (j & 7)), lds + (wm + j) * 8 + ((4 + g) ^ (j & 7))};
-    const int wrow = wn + (j >> 2) * V + (j & 3), wkey = (j & 3) | (j >> 2 & 1) << 2;
+    const int wrow = wn + (j >> 2) * 8 + (j & 3), wkey = (j & 3) | (j >> 2 & 1) << 2;
     const u32x4 *const wsrc[2] = {lds + 2 * BIG * 8 + wrow * 8 + (g ^ wkey), lds + 2 * BIG * 8 + wrow * 8 + ((4 + g) ^ wkey)};
     auto read_x = [&](Half &h, int i, int buf, int half) { h.v[i & 3][i >> 2] = xsrc[i >> 2][buf * (BIG * 8) + (half * 4 + (i & 3)) * 128]; };
-    auto read_w = [&](Half &h, int i, int buf, int half) { h.v[i & 3][i >> 2] = wsrc[i >> 2][buf * (BIG * 8) + (half * 4 + (i & 3)) * 32]; };
+    auto read_w = [&](Half &h, int i, int buf, int half) { h.v[i & 3][i >> 2] = wsrc[i >> 2][buf * (BIG * 8) + half * 512 + (i >> 1 & 1) * 256 + (i & 1) * 32]; };
 
     f32x4 acc[8][8];                                          // [w tile][x tile]
 #pragma unroll
@@ -437,29 +444,31 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     using Hi = std::integral_constant<int, 1>;
     Half x0, x1, w0, w1;
     // One k-tile from buffer `buf`; x0 and the first w half (wa) are in registers, the pieces of the next tile in xg, wg or on
-    // their way.  k2: where the tile after the next begins (past the end: zeros are fetched, and never read).
+    // their way.  k2: where the tile after the next begins (past the end: zeros are fetched, and never read).  The other
+    // buffer was last read before the barrier of the tile before, this one before the barrier here: its first pieces follow
+    // at once.  The pieces are spread over the whole tile, for a CU's address path takes 16 cycles for each (all in one
+    // quadrant: 5 % slower).
     auto tile = [&](int buf, int k2, Half &wa, Half &wb, auto ha, auto hb) {
         constexpr int WB = decltype(hb)::value;
-        const unsigned ko = k_offset(k2);
+        const unsigned ko = k_offset(k2), ko3 = k_offset(k2 + KT);
         multiply(wa, x0, ha, Lo{}, [&](int i) {
             if (i < 4) read_w(wb, 2 * i, buf, WB), read_w(wb, 2 * i + 1, buf, WB);
+            if (i % 2 == 0) move(4 + i / 2, buf ^ 1, ko);
         });
         multiply(wb, x0, hb, Lo{}, [&](int i) {
             if (i < 4) read_x(x1, 2 * i, buf, 1), read_x(x1, 2 * i + 1, buf, 1);
-            else stash_x(2 * i - 8, buf ^ 1), stash_x(2 * i - 7, buf ^ 1);
+            if (i % 2 == 0) move(8 + i / 2, buf ^ 1, ko);
         });
         multiply(wb, x1, hb, Hi{}, [&](int i) {
-            if (i < 4) stash_w(2 * i, buf ^ 1), stash_w(2 * i + 1, buf ^ 1);
-            else fetch_x(2 * i - 8, ko), fetch_x(2 * i - 7, ko);
+            if (i % 2 == 0) move(12 + i / 2, buf ^ 1, ko);
         });
         lds_barrier();
         multiply(wa, x1, ha, Hi{}, [&](int i) {
             if (i < 4) {
                 read_x(x0, 2 * i, buf ^ 1, 0), read_x(x0, 2 * i + 1, buf ^ 1, 0);
                 read_w(wb, 2 * i, buf ^ 1, WB), read_w(wb, 2 * i + 1, buf ^ 1, WB);
-            } else {
-                fetch_w(2 * i - 8, ko), fetch_w(2 * i - 7, ko);
             }
+            if (i % 2 == 0) move(i / 2, buf, ko3);
         });
     };
     const unsigned k0 = k_offset(0), k1 = k_offset(KT);
@@ -474,6 +483,9 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < 8; ++i) read_x(x0, i, 0, 0), read_w(w0, i, 0, 0);
+    const unsigned k2 = k_offset(2 * KT);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) move(i, 1, k2);
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 7" ::: "memory");                     // (the zeros just written to the accumulators: two states before their first use)
     __builtin_amdgcn_sched_barrier(0);
@@ -489,7 +501,7 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 
-    epilogue<8, V>(a, m0 + wm + j, n0 + wn + g * V, [&](int m, float (&v)[V]) { take_tile<8, 8>(acc, m, v); });
+    epilogue<8, V>(a, m0 + wm + j, n0 + wn + g * 8, [&](int m, float (&v)[V]) { take_tile<8, 8>(acc, m, v); });
 }
 
 template <int TYPE>
