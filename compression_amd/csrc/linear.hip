@@ -129,6 +129,12 @@ __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, i
     }
 }
 
+template <typename T>
+__device__ __forceinline__ void finish_one(const LinearArgs &a, int64_t m, int64_t n, float v) {
+    if (a.res) v += (float)((const T *)(a.res + m * a.rs))[n];
+    ((T *)(a.out + m * a.os))[n] = (T)v;
+}
+
 template <int MF, int V, typename Take>
 __device__ __forceinline__ void epilogue(const LinearArgs &a, int64_t row0, int64_t n, Take take) {
     if (n >= a.N) return;
@@ -521,6 +527,89 @@ int launch_big(mpc_ctx *ctx, LinearArgs a) {
     return MPC_OK;
 }
 
+// ---- few rows: the weights' bytes are all that counts -----------------------------------------------------------------------------
+// A workgroup takes 16 rows of w, its waves every WAVES-th k-tile of them, straight from memory into the registers of the
+// matrix instructions: no operand is used twice, so nothing goes through LDS but the waves' sums, which meet there in the
+// order of the waves.  UNITS k-tiles of a wave are in flight at once (64 KB and more per workgroup).
+template <int TYPE, int MF, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
+    constexpr int UNITS = 4;
+    __shared__ f32x4 part[WAVES * MF * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int j = lane & 15, g = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const char *w = a.w + (n0 + j < a.N ? n0 + j : a.N - 1) * a.ws + g * 16, *x[MF];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) x[m] = a.x + (m * 16 + j < a.M ? m * 16 + j : a.M - 1) * a.xs + g * 16;
+    f32x4 acc[MF];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) acc[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int units = (int)((a.K + KT - 1) / KT);
+    for (int first = wave; first < units; first += WAVES * UNITS) {
+        u32x4 wv[UNITS][2], xv[UNITS][MF][2];
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            const int u = first + i * WAVES;
+            const int64_t k = (int64_t)u * KT;
+            if (k + KT <= a.K) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    wv[i][c] = *(const u32x4_any *)(w + k + c * 64);
+#pragma unroll
+                    for (int m = 0; m < MF; ++m) xv[i][m][c] = *(const u32x4_any *)(x[m] + k + c * 64);
+                }
+            } else {                                          // the row's end, or past it: zeros
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int64_t left = a.K - k - c * 64 - g * 16;
+                    wv[i][c] = load_piece<Operand<TYPE>::BYTES>(w + k + c * 64, left);
+#pragma unroll
+                    for (int m = 0; m < MF; ++m) xv[i][m][c] = load_piece<Operand<TYPE>::BYTES>(x[m] + k + c * 64, left);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i)
+#pragma unroll
+            for (int m = 0; m < MF; ++m) {
+                if constexpr (TYPE == MPC_TYPE_E4M3) {
+                    acc[m] = Operand<TYPE>::mma(wv[i][0], wv[i][1], xv[i][m][0], xv[i][m][1], acc[m]);
+                } else {
+                    acc[m] = Operand<TYPE>::mma(wv[i][0], xv[i][m][0], acc[m]);
+                    acc[m] = Operand<TYPE>::mma(wv[i][1], xv[i][m][1], acc[m]);
+                }
+            }
+    }
+    // [wave][16 MF rows][16 columns]
+#pragma unroll
+    for (int m = 0; m < MF; ++m) part[(wave * MF + m) * 64 + j * 4 + g] = acc[m];
+    __syncthreads();
+    const float *sums = (const float *)part;
+    for (int t = tid; t < MF * 256; t += 64 * WAVES) {
+        const int64_t m = t >> 4, n = n0 + (t & 15);
+        if (m >= a.M || n >= a.N) continue;
+        float v[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) v[0] += sums[i * MF * 256 + t];
+        if (a.sx) v[0] *= a.sx[m] * a.sw[n];
+        if (a.bias) v[0] += a.bias[n];
+        activate<1>(v, a.act);
+        if (a.out_type == MPC_TYPE_F32) finish_one<float>(a, m, n, v[0]);
+        else if (a.out_type == MPC_TYPE_F16) finish_one<f16_t>(a, m, n, v[0]);
+        else finish_one<bf16_t>(a, m, n, v[0]);
+    }
+}
+
+template <int TYPE, int MF>
+int launch_rows(mpc_ctx *ctx, const LinearArgs &a) {
+    const int64_t blocks = mpc_cdiv(a.N, 16);
+    // up to a workgroup per CU: 16 waves, so that the CU's whole share of w is on its way; more: 8 waves, two workgroups a CU
+    if (blocks <= 256) linear_rows_kernel<TYPE, MF, 16><<<dim3((unsigned)blocks), dim3(1024), 0, ctx->stream>>>(a);
+    else linear_rows_kernel<TYPE, MF, 8><<<dim3((unsigned)blocks), dim3(512), 0, ctx->stream>>>(a);
+    MPC_CHECK_LAUNCH(ctx, "linear_rows");
+    return MPC_OK;
+}
+
 // 16-byte pieces everywhere, and offsets inside a tile that 30 bits hold
 bool big_possible(const LinearArgs &a) {
     return ((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.xs | (uintptr_t)a.ws | (uintptr_t)a.K) % 16 == 0 &&
@@ -529,7 +618,9 @@ bool big_possible(const LinearArgs &a) {
 
 template <int TYPE>
 int launch(mpc_ctx *ctx, const LinearArgs &a) {
-    if (big_possible(a) && mpc_cdiv(a.M, BIG) * mpc_cdiv(a.N, BIG) >= 256) return launch_big<TYPE>(ctx, a);
+    if (a.M <= 16) return launch_rows<TYPE, 1>(ctx, a);
+    if (a.M <= 32) return launch_rows<TYPE, 2>(ctx, a);
+    if (big_possible(a) && mpc_cdiv(a.M, BIG) * mpc_cdiv(a.N, BIG) >= 256 && a.K >= 2048) return launch_big<TYPE>(ctx, a);
     return launch_tiles<TYPE, 128, 128, 64, 64>(ctx, a);
 }
 
