@@ -223,7 +223,13 @@ def context_for(device) -> Context:
 
     if device.type != "cuda":
         raise MpcError(f"compression_amd runs on an MI355X only (got device '{device}'); there is no CPU path")
-    index = device.index if device.index is not None else torch.cuda.current_device()
+    return context_at(device.index if device.index is not None else torch.cuda.current_device())
+
+
+def context_at(index: int) -> Context:
+    """context_for, by the GPU's index."""
+    import torch
+
     ctx = _contexts.get(index)
     if ctx is None:
         ctx = _contexts[index] = Context(index, 0)

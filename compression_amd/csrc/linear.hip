@@ -31,6 +31,7 @@ struct LinearArgs {
     int out_type, act;
     int vec_out, vec_res;             // 16-byte accesses are possible
     int tiles_m, tiles_n;
+    float *partial;                   // [splits][M][N] sums, where K is split
 };
 
 // ---- epilogue ---------------------------------------------------------------------------------------------------------
@@ -204,143 +205,6 @@ __device__ __forceinline__ u32x4 load_piece(const char *p, int64_t left) {
 // ---- tiles through LDS --------------------------------------------------------------------------------------------------
 constexpr int KT = 128;               // bytes of a k-tile
 
-template <int TYPE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void linear_tile_kernel(LinearArgs a) {
-    constexpr int NT = 64 * (BM / WM) * (BN / WN);
-    constexpr int MF = WM / 16, NF = WN / 16, V = 4 * NF;
-    constexpr int XP = BM * 8 / NT, WP = BN * 8 / NT;             // 16-byte pieces per thread and tile
-    extern __shared__ u32x4 lds[];                                // 2 x [BM + BN rows][8 pieces]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int j = lane & 15, g = lane >> 4;
-    const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
-    const int64_t m0 = (int64_t)(blockIdx.x % a.tiles_m) * BM, n0 = (int64_t)(blockIdx.x / a.tiles_m) * BN;
-
-    // Piece p of row r lies at slot p ^ key(r): the 16 rows that one instruction reads at the same p then spread over the banks.
-    auto xkey = [](int r) { return r & 7; };
-    auto wkey = [](int r) { return (r & 3) | (r >> 3 & 1) << 2; };
-
-    const int p = tid & 7;
-    const char *xp[XP], *wp[WP];
-#pragma unroll
-    for (int i = 0; i < XP; ++i) {
-        const int64_t r = m0 + tid / 8 + i * (NT / 8);
-        xp[i] = a.x + (r < a.M ? r : a.M - 1) * a.xs + p * 16;
-    }
-#pragma unroll
-    for (int i = 0; i < WP; ++i) {
-        const int64_t r = n0 + tid / 8 + i * (NT / 8);
-        wp[i] = a.w + (r < a.N ? r : a.N - 1) * a.ws + p * 16;
-    }
-    u32x4 xr[XP], wr[WP];
-    auto fetch = [&](int64_t k) {
-        if (k + KT <= a.K) {
-#pragma unroll
-            for (int i = 0; i < XP; ++i) xr[i] = *(const u32x4_any *)(xp[i] + k);
-#pragma unroll
-            for (int i = 0; i < WP; ++i) wr[i] = *(const u32x4_any *)(wp[i] + k);
-        } else {
-            const int64_t left = a.K - k - p * 16;
-#pragma unroll
-            for (int i = 0; i < XP; ++i) xr[i] = load_piece<Operand<TYPE>::BYTES>(xp[i] + k, left);
-#pragma unroll
-            for (int i = 0; i < WP; ++i) wr[i] = load_piece<Operand<TYPE>::BYTES>(wp[i] + k, left);
-        }
-    };
-    auto stash = [&](int buf) {
-        u32x4 *x = lds + buf * (BM + BN) * 8, *w = x + BM * 8;
-#pragma unroll
-        for (int i = 0; i < XP; ++i) {
-            const int r = tid / 8 + i * (NT / 8);
-            x[r * 8 + (p ^ xkey(r))] = xr[i];
-        }
-#pragma unroll
-        for (int i = 0; i < WP; ++i) {
-            const int r = tid / 8 + i * (NT / 8);
-            w[r * 8 + (p ^ wkey(r))] = wr[i];
-        }
-    };
-
-    f32x4 acc[NF][MF];
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-        for (int m = 0; m < MF; ++m) acc[f][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    fetch(0);
-    stash(0);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t k = 0; k < a.K; k += KT, buf ^= 1) {
-        const bool more = k + KT < a.K;
-        if (more) fetch(k + KT);
-        const u32x4 *x = lds + buf * (BM + BN) * 8, *w = x + BM * 8;
-        auto xfrag = [&](int m, int q) {
-            const int r = wm + m * 16 + j;
-            return x[r * 8 + (q ^ xkey(r))];
-        };
-        auto wfrag = [&](int f, int q) {
-            const int r = wn + (f >> 1) * 32 + (j >> 2) * 8 + (f & 1) * 4 + (j & 3);
-            return w[r * 8 + (q ^ wkey(r))];
-        };
-        if constexpr (TYPE == MPC_TYPE_E4M3) {
-            u32x4 b0[MF], b1[MF];
-#pragma unroll
-            for (int m = 0; m < MF; ++m) b0[m] = xfrag(m, g), b1[m] = xfrag(m, g + 4);
-#pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                const u32x4 a0 = wfrag(f, g), a1 = wfrag(f, g + 4);
-#pragma unroll
-                for (int m = 0; m < MF; ++m) acc[f][m] = Operand<TYPE>::mma(a0, a1, b0[m], b1[m], acc[f][m]);
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                u32x4 b[MF];
-#pragma unroll
-                for (int m = 0; m < MF; ++m) b[m] = xfrag(m, 4 * s + g);
-#pragma unroll
-                for (int f = 0; f < NF; ++f) {
-                    const u32x4 w4 = wfrag(f, 4 * s + g);
-#pragma unroll
-                    for (int m = 0; m < MF; ++m) acc[f][m] = Operand<TYPE>::mma(w4, b[m], acc[f][m]);
-                }
-            }
-        }
-        if (more) stash(buf ^ 1);            // (the other buffer was last read before the previous barrier)
-        __syncthreads();
-    }
-
-    epilogue<MF, V>(a, m0 + wm + j, n0 + wn + g * 8, [&](int m, float (&v)[V]) { take_tile<MF, NF>(acc, m, v); });
-}
-
-template <int TYPE, int BM, int BN, int WM, int WN>
-int launch_tiles(mpc_ctx *ctx, LinearArgs a) {
-    constexpr size_t lds = 2 * (BM + BN) * KT;
-    auto kern = linear_tile_kernel<TYPE, BM, BN, WM, WN>;
-    static bool attr_set[MPC_MAX_DEVICES] = {};
-    bool &attr_done = attr_set[ctx->device];
-    if (lds > 48 * 1024 && !attr_done) {
-        MPC_HIP(ctx, hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        attr_done = true;
-    }
-    const int64_t tm = mpc_cdiv(a.M, BM), tn = mpc_cdiv(a.N, BN);
-    MPC_REQUIRE(ctx, tm * tn < (1ll << 31), "linear: too many tiles");
-    a.tiles_m = (int)tm;
-    a.tiles_n = (int)tn;
-    kern<<<dim3((unsigned)(tm * tn)), dim3(64 * (BM / WM) * (BN / WN)), lds, ctx->stream>>>(a);
-    MPC_CHECK_LAUNCH(ctx, "linear_tile");
-    return MPC_OK;
-}
-
-// ---- large products: 256 x 256 tiles, one workgroup per CU -------------------------------------------------------------------
-// Four waves, each 128 x 128 outputs in 256 accumulator registers: a wave then reads 32 KB of LDS per k-tile for 2048 cycles
-// of matrix instructions (the four of a CU 64 bytes a cycle; waves of 64 x 64 would need all 128 that LDS delivers).  With one
-// wave per SIMD nothing else hides its latencies, so they are hidden in the wave itself: a k-tile is four quadrants of
-// 64 x 64, and while one multiplies, the operands of the next come from LDS, the pieces of the next k-tile go from
-// registers to the other LDS buffer and those of the one after leave for memory.  The last quadrant of a tile shares no
-// operand with the first of the next, so the order of the w halves alternates from tile to tile.
-constexpr int BIG = 256;
-
 __device__ __forceinline__ void lds_barrier() {               // LDS accesses done, then the barrier; memory loads stay in flight
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -357,7 +221,239 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int &tm
     tn = in / rows;
 }
 
+// 16 bytes that begin `sh` bytes before the piece wanted (the row ends inside it, or before it): the piece, zeros behind the row
+__device__ __forceinline__ u32x4 row_end(u32x4 v, int sh) {
+    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+    u64x2 t = __builtin_bit_cast(u64x2, v);
+    if (sh >= 16) t[0] = t[1] = 0;
+    else if (sh >= 8) t[0] = t[1] >> (8 * sh - 64), t[1] = 0;
+    else if (sh > 0) t[0] = t[0] >> (8 * sh) | t[1] << (64 - 8 * sh), t[1] >>= 8 * sh;
+    return __builtin_bit_cast(u32x4, t);
+}
+
+// A tile's rows of an operand as a buffer: a row past the last gets an offset past the end, and such a load gives zeros.
+constexpr unsigned NO_ROW = 0x80000000u;
+constexpr int64_t TILE_BYTES = 1ll << 30;                         // most that a tile's rows may span (the host checks)
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t tile_buffer(const char *base, int rows, int64_t stride, int64_t K) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)((rows - 1) * stride + K), 0x00020000);
+}
+__device__ __forceinline__ u32x4 buffer_piece(rsrc_t r, unsigned offset) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
+}
+
+// Workgroup (tile, split): BM x BN outputs over the split's k-tiles.  DEPTH k-tiles are on their way in registers while one
+// is worked on from LDS, so a tile of few rows, whose matrix instructions do not cover a memory access, is not bound by
+// it.  Operand rows may begin at any element, and are at least 16 bytes long.  The last k-tile, if the row ends inside
+// it, comes by itself behind the others: a piece past the row's end is loaded from its last 16 bytes and shifted.
+template <int TYPE, int BM, int BN, int WM, int WN, int DEPTH, int PER_SIMD>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_tile_kernel(LinearArgs a) {
+    constexpr int NT = 64 * (BM / WM) * (BN / WN), TURN = DEPTH % 2 ? 2 * DEPTH : DEPTH;
+    constexpr int MF = WM / 16, NF = WN / 16, V = 4 * NF;
+    constexpr int XP = BM * 8 / NT, WP = BN * 8 / NT;             // 16-byte pieces per thread and tile
+    extern __shared__ u32x4 lds[];                                // 2 x [BM + BN rows][8 pieces]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int j = lane & 15, g = lane >> 4;
+    const int wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int rows_x = (int)(a.M - m0 < BM ? a.M - m0 : BM), rows_w = (int)(a.N - n0 < BN ? a.N - n0 : BN);
+    const rsrc_t xb = tile_buffer(a.x + m0 * a.xs, rows_x, a.xs, a.K), wb = tile_buffer(a.w + n0 * a.ws, rows_w, a.ws, a.K);
+    // this split's k-tiles: T whole ones, and in the last split the one in which the rows end
+    const int K = (int)a.K, whole = K / KT, all = (K + KT - 1) / KT;
+    const int t0 = (int)((int64_t)all * blockIdx.y / gridDim.y), t1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
+    const int T = (t1 < whole ? t1 : whole) - t0;
+
+    // Piece p of row r lies at slot p ^ key(r): the 16 rows that one instruction reads at the same p then spread over the banks.
+    auto xkey = [](int r) { return r & 7; };
+    auto wkey = [](int r) { return (r & 3) | (r >> 3 & 1) << 2; };
+    const int p = tid & 7, r0 = tid >> 3;
+    unsigned xo[XP], wo[WP];
+#pragma unroll
+    for (int i = 0; i < XP; ++i) xo[i] = r0 + i * (NT / 8) < rows_x ? (unsigned)((r0 + i * (NT / 8)) * a.xs) : NO_ROW;
+#pragma unroll
+    for (int i = 0; i < WP; ++i) wo[i] = r0 + i * (NT / 8) < rows_w ? (unsigned)((r0 + i * (NT / 8)) * a.ws) : NO_ROW;
+    u32x4 xr[DEPTH][XP], wr[DEPTH][WP];
+    auto fetch = [&](int slot, int t) {                           // (past the row's end: its last piece)
+        const int at = (t0 + t) * KT + p * 16, off = at < K - 16 ? at : K - 16;
+#pragma unroll
+        for (int i = 0; i < XP; ++i) xr[slot][i] = buffer_piece(xb, xo[i] + off);
+#pragma unroll
+        for (int i = 0; i < WP; ++i) wr[slot][i] = buffer_piece(wb, wo[i] + off);
+    };
+    auto stash = [&](int slot, int buf) {
+        u32x4 *x = lds + buf * (BM + BN) * 8, *w = x + BM * 8;
+#pragma unroll
+        for (int i = 0; i < XP; ++i) {
+            const int r = r0 + i * (NT / 8);
+            x[r * 8 + (p ^ xkey(r))] = xr[slot][i];
+        }
+#pragma unroll
+        for (int i = 0; i < WP; ++i) {
+            const int r = r0 + i * (NT / 8);
+            w[r * 8 + (p ^ wkey(r))] = wr[slot][i];
+        }
+    };
+    f32x4 acc[NF][MF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int m = 0; m < MF; ++m) acc[f][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // One k-tile from LDS buffer buf.  Its operands are asked for first, all of them: their way from LDS is paid once, not once
+    // per group of instructions; `beside` follows them.
+    auto multiply = [&](int buf, auto beside) {
+        const u32x4 *x = lds + buf * (BM + BN) * 8, *w = x + BM * 8;
+        u32x4 xv[2][MF], wv[2][NF];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int m = 0; m < MF; ++m) {
+                const int r = wm + m * 16 + j;
+                xv[c][m] = x[r * 8 + ((4 * c + g) ^ xkey(r))];
+            }
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const int r = wn + (f >> 1) * 32 + (j >> 2) * 8 + (f & 1) * 4 + (j & 3);
+                wv[c][f] = w[r * 8 + ((4 * c + g) ^ wkey(r))];
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        beside();
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (TYPE == MPC_TYPE_E4M3) {
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int m = 0; m < MF; ++m) acc[f][m] = Operand<TYPE>::mma(wv[0][f], wv[1][f], xv[0][m], xv[1][m], acc[f][m]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int f = 0; f < NF; ++f)
+#pragma unroll
+                    for (int m = 0; m < MF; ++m) acc[f][m] = Operand<TYPE>::mma(wv[c][f], xv[c][m], acc[f][m]);
+        }
+    };
+    // Tile t from LDS buffer t & 1; tile t + 1 waits in slot (t + 1) % DEPTH.  Tiles past the last are fetched and stored like
+    // the others, and never read: a fetch under a condition would make the compiler wait for every load in flight, since it
+    // could not count on the younger ones.
+    auto step = [&](int buf, int slot, int t) {
+        multiply(buf, [&] {
+            stash(slot, buf ^ 1);                                 // (last read before the previous barrier)
+            fetch(slot, t + 1 + DEPTH);
+        });
+        lds_barrier();
+    };
+    if (T > 0) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) fetch(d, d);
+        stash(0, 0);
+        fetch(0, DEPTH);
+        lds_barrier();
+        for (int t = 0;; t += TURN) {
+#pragma unroll
+            for (int i = 0; i < TURN; ++i) {
+                if (t + i >= T) goto done;
+                step(i & 1, (i + 1) % DEPTH, t + i);
+            }
+        }
+    }
+done:
+    if (t1 > whole) {                                             // the tile in which the rows end
+        fetch(0, whole - t0);
+        const int over = whole * KT + p * 16 - (K - 16), sh = over < 0 ? 0 : over > 16 ? 16 : over;
+#pragma unroll
+        for (int i = 0; i < XP; ++i) xr[0][i] = row_end(xr[0][i], sh);
+#pragma unroll
+        for (int i = 0; i < WP; ++i) wr[0][i] = row_end(wr[0][i], sh);
+        stash(0, 0);
+        lds_barrier();
+        multiply(0, [] {});
+    }
+    if (gridDim.y > 1) {                                          // the sums as they are; linear_join_kernel finishes them
+        LinearArgs sums = a;
+        sums.sx = sums.sw = sums.bias = nullptr;
+        sums.res = nullptr;
+        sums.out = (char *)(a.partial + (int64_t)blockIdx.y * a.M * a.N);
+        sums.os = a.N * 4;
+        sums.out_type = MPC_TYPE_F32, sums.act = MPC_ACT_NONE;
+        sums.vec_out = a.N % 4 == 0;
+        finish_rows<float, MF, V>(sums, m0 + wm + j, n0 + wn + g * 8, [&](int m, float (&v)[V]) { take_tile<MF, NF>(acc, m, v); });
+        return;
+    }
+    epilogue<MF, V>(a, m0 + wm + j, n0 + wn + g * 8, [&](int m, float (&v)[V]) { take_tile<MF, NF>(acc, m, v); });
+}
+
+// Adds up the splits' sums, in their order, and finishes: four columns of a row per thread.
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int splits) {
+    const int64_t per_row = (a.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.M * per_row) return;
+    const int64_t m = i / per_row, n = i % per_row * 4, plane = a.M * a.N;
+    const float *s = a.partial + m * a.N + n;
+    const bool whole = a.N % 4 == 0;                              // (then the rows are aligned as well)
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int z = 0; z < splits; ++z) {
+        if (whole) {
+            const f32x4 t = *(const f32x4 *)(s + z * plane);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] += t[c];
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (n + c < a.N) v[c] += s[z * plane + c];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (n + c >= a.N) break;
+        if (a.sx) v[c] *= a.sx[m] * a.sw[n + c];
+        if (a.bias) v[c] += a.bias[n + c];
+    }
+    activate<4>(v, a.act);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (n + c >= a.N) break;
+        if (a.out_type == MPC_TYPE_F32) finish_one<float>(a, m, n + c, v[c]);
+        else if (a.out_type == MPC_TYPE_F16) finish_one<f16_t>(a, m, n + c, v[c]);
+        else finish_one<bf16_t>(a, m, n + c, v[c]);
+    }
+}
+
+template <int TYPE, int BM, int BN, int WM, int WN, int DEPTH, int PER_SIMD>
+int launch_tiles(mpc_ctx *ctx, LinearArgs a, int splits) {
+    constexpr size_t lds = 2 * (BM + BN) * KT;
+    auto kern = linear_tile_kernel<TYPE, BM, BN, WM, WN, DEPTH, PER_SIMD>;
+    static bool attr_set[MPC_MAX_DEVICES] = {};
+    bool &attr_done = attr_set[ctx->device];
+    if (lds > 48 * 1024 && !attr_done) {
+        MPC_HIP(ctx, hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        attr_done = true;
+    }
+    const int64_t tm = mpc_cdiv(a.M, BM), tn = mpc_cdiv(a.N, BN);
+    MPC_REQUIRE(ctx, tm * tn < (1ll << 30), "linear: too many tiles");
+    a.tiles_m = (int)tm;
+    a.tiles_n = (int)tn;
+    kern<<<dim3((unsigned)(tm * tn), (unsigned)splits), dim3(64 * (BM / WM) * (BN / WN)), lds, ctx->stream>>>(a);
+    MPC_CHECK_LAUNCH(ctx, "linear_tile");
+    if (splits > 1) {
+        const int64_t blocks = mpc_cdiv(a.M * ((a.N + 3) / 4), 256);
+        MPC_REQUIRE(ctx, blocks < (1ll << 31), "linear: too many outputs to join");
+        linear_join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, ctx->stream>>>(a, splits);
+        MPC_CHECK_LAUNCH(ctx, "linear_join");
+    }
+    return MPC_OK;
+}
+
+// ---- large products: 256 x 256 tiles, one workgroup per CU -------------------------------------------------------------------
+// Four waves, each 128 x 128 outputs in 256 accumulator registers: a wave then reads 32 KB of LDS per k-tile for 2048 cycles
+// of matrix instructions (the four of a CU 64 bytes a cycle; waves of 64 x 64 would need all 128 that LDS delivers).  With one
+// wave per SIMD nothing else hides its latencies, so they are hidden in the wave itself: a k-tile is four quadrants of
+// 64 x 64, and while one multiplies, the operands of the next come from LDS, the pieces of the next k-tile go from
+// registers to the other LDS buffer and those of the one after leave for memory.  The last quadrant of a tile shares no
+// operand with the first of the next, so the order of the w halves alternates from tile to tile.
+constexpr int BIG = 256;
 
 // c += a b with c in accumulation registers, in place.  All 256 of them hold sums here; through the builtin the compiler moves
 // sums from register to register (a result need not go where its input was), with none left to move them through: twice as
@@ -386,11 +482,9 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     const int64_t m0 = (int64_t)tm * BIG, n0 = (int64_t)tn * BIG;
     const int rows_x = (int)(a.M - m0 < BIG ? a.M - m0 : BIG), rows_w = (int)(a.N - n0 < BIG ? a.N - n0 : BIG);
 
-    // Pieces come by buffer loads with the tile's own rows as bounds: a row past the last, or a piece past K (a multiple of 16
-    // bytes here), gets an offset past the end, and such a load gives zeros.
-    constexpr unsigned NO_ROW = 0x80000000u, NO_K = 0x40000000u;   // (the tile ends below 2^30: the host checks)
-    const rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.x + m0 * a.xs), 0, (int)((rows_x - 1) * a.xs + a.K), 0x00020000);
-    const rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + n0 * a.ws), 0, (int)((rows_w - 1) * a.ws + a.K), 0x00020000);
+    // A piece past K (a multiple of 16 bytes here) gets an offset past the end, like a row past the last.
+    constexpr unsigned NO_K = 0x40000000u;
+    const rsrc_t xr = tile_buffer(a.x + m0 * a.xs, rows_x, a.xs, a.K), wr = tile_buffer(a.w + n0 * a.ws, rows_w, a.ws, a.K);
     const int p = tid & 7, r0 = tid >> 3;
     unsigned xo[8], wo[8];
 #pragma unroll
@@ -402,8 +496,8 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     u32x4 xg[8], wg[8];
     const int K = (int)a.K;
     auto k_offset = [&](int k) { return k + p * 16 < K ? (unsigned)k : NO_K; };
-    auto fetch_x = [&](int i, unsigned ko) { xg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(xr, xo[i] + ko, 0, 0)); };
-    auto fetch_w = [&](int i, unsigned ko) { wg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wr, wo[i] + ko, 0, 0)); };
+    auto fetch_x = [&](int i, unsigned ko) { xg[i] = buffer_piece(xr, xo[i] + ko); };
+    auto fetch_w = [&](int i, unsigned ko) { wg[i] = buffer_piece(wr, wo[i] + ko); };
     // LDS slots, as in the kernel above: piece p of row r at p ^ key(r); rows of w are read interleaved, so its
     // key takes bit 3 of the row.  [x buffer 0][x buffer 1][w buffer 0][w buffer 1], each 256 rows of 8 pieces.
     u32x4 *const xdst = lds + r0 * 8 + (p ^ (r0 & 7));
@@ -530,17 +624,18 @@ int launch_big(mpc_ctx *ctx, LinearArgs a) {
 // ---- few rows: the weights' bytes are all that counts -----------------------------------------------------------------------------
 // A workgroup takes 16 rows of w, its waves every WAVES-th k-tile of them, straight from memory into the registers of the
 // matrix instructions: no operand is used twice, so nothing goes through LDS but the waves' sums, which meet there in the
-// order of the waves.  UNITS k-tiles of a wave are in flight at once (64 KB and more per workgroup).
+// order of the waves.  UNITS k-tiles of a wave are in flight at once (64 KB and more per workgroup).  More rows than
+// MF tiles take more workgroups (only for the rows that no other kernel takes: see plan_for).
 template <int TYPE, int MF, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
     constexpr int UNITS = 4;
     __shared__ f32x4 part[WAVES * MF * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 15, g = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int64_t n0 = (int64_t)(blockIdx.x % a.tiles_n) * 16, m0 = (int64_t)(blockIdx.x / a.tiles_n) * (16 * MF);
     const char *w = a.w + (n0 + j < a.N ? n0 + j : a.N - 1) * a.ws + g * 16, *x[MF];
 #pragma unroll
-    for (int m = 0; m < MF; ++m) x[m] = a.x + (m * 16 + j < a.M ? m * 16 + j : a.M - 1) * a.xs + g * 16;
+    for (int m = 0; m < MF; ++m) x[m] = a.x + (m0 + m * 16 + j < a.M ? m0 + m * 16 + j : a.M - 1) * a.xs + g * 16;
     f32x4 acc[MF];
 #pragma unroll
     for (int m = 0; m < MF; ++m) acc[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -586,7 +681,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
     __syncthreads();
     const float *sums = (const float *)part;
     for (int t = tid; t < MF * 256; t += 64 * WAVES) {
-        const int64_t m = t >> 4, n = n0 + (t & 15);
+        const int64_t m = m0 + (t >> 4), n = n0 + (t & 15);
         if (m >= a.M || n >= a.N) continue;
         float v[1] = {0.0f};
 #pragma unroll
@@ -601,8 +696,10 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
 }
 
 template <int TYPE, int MF>
-int launch_rows(mpc_ctx *ctx, const LinearArgs &a) {
-    const int64_t blocks = mpc_cdiv(a.N, 16);
+int launch_rows(mpc_ctx *ctx, LinearArgs a) {
+    const int64_t tiles_n = mpc_cdiv(a.N, 16), blocks = tiles_n * mpc_cdiv(a.M, 16 * MF);
+    MPC_REQUIRE(ctx, blocks < (1ll << 31), "linear: too many tiles");
+    a.tiles_n = (int)tiles_n;
     // up to a workgroup per CU: 16 waves, so that the CU's whole share of w is on its way; more: 8 waves, two workgroups a CU
     if (blocks <= 256) linear_rows_kernel<TYPE, MF, 16><<<dim3((unsigned)blocks), dim3(1024), 0, ctx->stream>>>(a);
     else linear_rows_kernel<TYPE, MF, 8><<<dim3((unsigned)blocks), dim3(512), 0, ctx->stream>>>(a);
@@ -610,18 +707,36 @@ int launch_rows(mpc_ctx *ctx, const LinearArgs &a) {
     return MPC_OK;
 }
 
-// 16-byte pieces everywhere, and offsets inside a tile that 30 bits hold
+// 16-byte pieces everywhere
 bool big_possible(const LinearArgs &a) {
-    return ((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.xs | (uintptr_t)a.ws | (uintptr_t)a.K) % 16 == 0 &&
-           BIG * a.xs + a.K < (1ll << 30) && BIG * a.ws + a.K < (1ll << 30) && mpc_cdiv(a.M, BIG) * mpc_cdiv(a.N, BIG) < (1ll << 31);
+    return ((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.xs | (uintptr_t)a.ws | (uintptr_t)a.K) % 16 == 0;
+}
+
+// ---- which kernel ---------------------------------------------------------------------------------------------------------------
+enum { PLAN_ROWS, PLAN_SMALL, PLAN_MIDDLE, PLAN_BIG };
+struct Plan {
+    int kind, splits;
+};
+
+Plan plan_for(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {     // the last three in bytes
+    // (rows shorter than a piece, or so far apart that a tile's do not fit a buffer: the kernel that addresses each by itself)
+    if (M <= 32 || K < 16 || BIG * xs + K > TILE_BYTES || BIG * ws + K > TILE_BYTES) return {PLAN_ROWS, 1};
+    const int64_t big = mpc_cdiv(M, BIG) * mpc_cdiv(N, BIG), middle = mpc_cdiv(M, 128) * mpc_cdiv(N, 128);
+    if (big >= 256 && K >= 2048) return {PLAN_BIG, 1};
+    if (middle >= 200) return {PLAN_MIDDLE, 1};
+    const int64_t small = mpc_cdiv(M, 64) * mpc_cdiv(N, 64), k_tiles = mpc_cdiv(K, KT);
+    int splits = 1;
+    while (splits < 16 && small * splits * 2 <= 1024 && k_tiles / (splits * 2) >= 8) splits *= 2;
+    return {PLAN_SMALL, splits};
 }
 
 template <int TYPE>
 int launch(mpc_ctx *ctx, const LinearArgs &a) {
-    if (a.M <= 16) return launch_rows<TYPE, 1>(ctx, a);
-    if (a.M <= 32) return launch_rows<TYPE, 2>(ctx, a);
-    if (big_possible(a) && mpc_cdiv(a.M, BIG) * mpc_cdiv(a.N, BIG) >= 256 && a.K >= 2048) return launch_big<TYPE>(ctx, a);
-    return launch_tiles<TYPE, 128, 128, 64, 64>(ctx, a);
+    const Plan plan = plan_for(a.M, a.N, a.K, a.xs, a.ws);
+    if (plan.kind == PLAN_ROWS) return a.M <= 16 ? launch_rows<TYPE, 1>(ctx, a) : launch_rows<TYPE, 2>(ctx, a);
+    if (plan.kind == PLAN_BIG && big_possible(a)) return launch_big<TYPE>(ctx, a);
+    if (plan.kind == PLAN_SMALL) return launch_tiles<TYPE, 64, 64, 32, 32, 4, 3>(ctx, a, plan.splits);
+    return launch_tiles<TYPE, 128, 128, 64, 64, 2, 2>(ctx, a, 1);
 }
 
 bool linear_desc_ok(const mpc_linear_desc &d) {
@@ -636,8 +751,10 @@ bool linear_desc_ok(const mpc_linear_desc &d) {
 }  // namespace
 
 extern "C" size_t mpc_linear_workspace_bytes(const mpc_linear_desc *desc) {
-    (void)desc;
-    return 0;
+    if (!desc || !linear_desc_ok(*desc) || desc->M == 0) return 0;
+    const int ib = mpc_type_bytes(desc->in_type);
+    const Plan plan = plan_for(desc->M, desc->N, desc->K * ib, desc->x_stride * ib, desc->w_stride * ib);
+    return plan.splits > 1 ? (size_t)plan.splits * desc->M * desc->N * sizeof(float) : 0;
 }
 
 extern "C" int mpc_linear_forward(mpc_ctx *ctx, const mpc_linear_desc *desc, const void *x, const float *x_scale, const void *w,
@@ -652,7 +769,9 @@ extern "C" int mpc_linear_forward(mpc_ctx *ctx, const mpc_linear_desc *desc, con
     MPC_REQUIRE(ctx, x && w && out, "linear: null pointer");
     const bool eight = d.in_type == MPC_TYPE_E4M3;
     MPC_REQUIRE(ctx, (x_scale != nullptr) == eight && (w_scale != nullptr) == eight, "linear: scales go with e4m3 operands, both of them");
-    MPC_REQUIRE(ctx, workspace_bytes >= mpc_linear_workspace_bytes(desc), "linear: workspace of %zu bytes", workspace_bytes);
+    const size_t need = mpc_linear_workspace_bytes(desc);
+    MPC_REQUIRE(ctx, workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
+                "linear: workspace of %zu bytes, %zu needed, 16-byte aligned", workspace_bytes, need);
     const int ib = mpc_type_bytes(d.in_type), ob = mpc_type_bytes(d.out_type);
     MPC_REQUIRE(ctx, ((uintptr_t)x | (uintptr_t)w) % ib == 0 && ((uintptr_t)out | (uintptr_t)residual) % ob == 0, "linear: misaligned pointer");
     LinearArgs a{};
@@ -665,7 +784,7 @@ extern "C" int mpc_linear_forward(mpc_ctx *ctx, const mpc_linear_desc *desc, con
     a.out_type = d.out_type, a.act = d.act;
     a.vec_out = (uintptr_t)out % 16 == 0 && a.os % 16 == 0;
     a.vec_res = (uintptr_t)residual % 16 == 0 && a.rs % 16 == 0;
-    (void)workspace;
+    a.partial = (float *)workspace;
     if (d.in_type == MPC_TYPE_F16) return launch<MPC_TYPE_F16>(ctx, a);
     if (d.in_type == MPC_TYPE_BF16) return launch<MPC_TYPE_BF16>(ctx, a);
     return launch<MPC_TYPE_E4M3>(ctx, a);

@@ -304,30 +304,24 @@ def _rows(t: torch.Tensor, name: str) -> Tuple[int, int]:
     return rows, step
 
 
-def _same_gpu(x: torch.Tensor, **others):
-    if not x.is_cuda:
+def _gpu_of(x: torch.Tensor, *others) -> int:
+    """Index of the GPU that x and the others that are not None live on."""
+    index = x.get_device()
+    if index < 0:
         raise MpcError(f"tensors must live on the GPU (got {x.device}); compression_amd has no CPU path")
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise MpcError(f"{name} is on {t.device}, the input on {x.device}")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise MpcError(f"operands on {x.device} and on {t.device}: all must be on one GPU")
+    return index
 
 
 def _addr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _call(name: str, device, entry: str, *args, **meta):
-    """One library call, timed under `name` if a Profiler is on (its context manager costs as much as the launch of a small
-    call, so it is left out otherwise)."""
-    if PROFILER is None:
-        context_for(device).call(entry, *args)
-    else:
-        with _timed(name, **meta):
-            context_for(device).call(entry, *args)
-
-
-def _vector(t: Optional[torch.Tensor], n: int, name: str):
-    if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
+# The wrappers below look a little bare: a call of a few rows takes the GPU 5-8 microseconds, and Python about as long.
+def _vector(t: torch.Tensor, n: int, name: str):
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
         raise MpcError(f"{name} must be {n} contiguous float32 values, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -340,27 +334,36 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     v ~ q * scale, what `linear` takes as x and x_scale.  With a residual h (x's type, rounded once; the norm is taken of
     the unrounded sum) is returned behind them: (v, h) or (q, scale, h).  Rows of zeros have scale 1.  Values only, like the
     rest of the library: no autograd graph."""
-    _same_gpu(x, weight=weight, residual=residual)
-    if x.dtype not in _ROW_TYPES:
-        raise MpcError(f"rms_norm: x must be float32, float16 or bfloat16 (got {x.dtype})")
+    index = _gpu_of(x, weight, residual)
+    dtype = x.dtype
+    t = _ROW_TYPES.get(dtype)
+    if t is None:
+        raise MpcError(f"rms_norm: x must be float32, float16 or bfloat16 (got {dtype})")
     rows, xs = _rows(x, "x")
     C = x.shape[-1]
-    _vector(weight, C, "weight")
-    rs = 0
+    if weight is not None:
+        _vector(weight, C, "weight")
+    h, rs = None, 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise MpcError(f"rms_norm: residual {residual.dtype} {tuple(residual.shape)} does not match x {x.dtype} {tuple(x.shape)}")
+        if residual.shape != x.shape or residual.dtype != dtype:
+            raise MpcError(f"rms_norm: residual {residual.dtype} {tuple(residual.shape)} does not match x {dtype} {tuple(x.shape)}")
         _, rs = _rows(residual, "residual")
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if quantize else x.dtype, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quantize else None
-    t = _ROW_TYPES[x.dtype]
+        h = x.new_empty(x.shape)
+    if quantize:
+        y, scale = x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    else:
+        y, scale = x.new_empty(x.shape), None
     if rows:
-        _call("rms_norm", x.device, "mpc_rms_norm", x.data_ptr(), xs, _addr(residual), rs, _addr(weight), rows, C, eps, t, _addr(h),
-              y.data_ptr(), _lib.MPC_TYPE_E4M3 if quantize else t, _addr(scale),
-              bytes=float(x.numel()) * (x.element_size() * (1 if residual is None else 3) + y.element_size()))
-    out = ((y, scale) if quantize else (y,)) + (() if h is None else (h,))
-    return out if len(out) > 1 else y
+        args = (x.data_ptr(), xs, _addr(residual), rs, _addr(weight), rows, C, eps, t, _addr(h), y.data_ptr(),
+                _lib.MPC_TYPE_E4M3 if quantize else t, _addr(scale))
+        if PROFILER is None:
+            _lib.context_at(index).call("mpc_rms_norm", *args)
+        else:
+            with _timed("rms_norm", bytes=float(x.numel()) * (x.element_size() * (1 if h is None else 3) + y.element_size())):
+                _lib.context_at(index).call("mpc_rms_norm", *args)
+    if quantize:
+        return (y, scale) if h is None else (y, scale, h)
+    return y if h is None else (y, h)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: int = _lib.MPC_ACT_NONE,
@@ -373,49 +376,60 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     bring their scales, fp32: x_scale [...] (one per row) and weight_scale [N]; 16-bit ones have none.  out_dtype: fp32,
     fp16 or bf16; default the residual's type, else x's, and fp16 for e4m3 operands.  Sums and epilogue in fp32, one
     rounding at the end.  Values only: no autograd graph."""
-    _same_gpu(x, weight=weight, bias=bias, residual=residual, x_scale=x_scale, weight_scale=weight_scale)
-    if x.dtype not in _OPERAND_TYPES or weight.dtype != x.dtype:
+    index = _gpu_of(x, weight, bias, residual, x_scale, weight_scale)
+    t = _OPERAND_TYPES.get(x.dtype)
+    if t is None or weight.dtype != x.dtype:
         raise MpcError(f"linear: x and weight must both be float16, bfloat16 or float8_e4m3fn (got {x.dtype}, {weight.dtype})")
     if act not in _LINEAR_ACTS:
         raise MpcError(f"linear: activation {act} is not one of {_LINEAR_ACTS}")
-    if weight.dim() != 2 or weight.shape[0] == 0 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
-        raise MpcError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
+    xshape = x.shape
+    if weight.dim() != 2 or weight.shape[0] == 0 or len(xshape) == 0 or xshape[-1] != weight.shape[1]:
+        raise MpcError(f"linear: x {tuple(xshape)} and weight {tuple(weight.shape)} do not fit")
     M, xs = _rows(x, "x")
     N, ws = _rows(weight, "weight")
-    eight = x.dtype == torch.float8_e4m3fn
+    K = xshape[-1]
+    eight = t == _lib.MPC_TYPE_E4M3
     if eight != (x_scale is not None) or eight != (weight_scale is not None):
         raise MpcError("linear: e4m3 operands need x_scale and weight_scale, 16-bit operands take none")
-    _vector(bias, N, "bias")
-    _vector(x_scale, M, "x_scale")
-    _vector(weight_scale, N, "weight_scale")
+    if eight:
+        _vector(x_scale, M, "x_scale")
+        _vector(weight_scale, N, "weight_scale")
+    if bias is not None:
+        _vector(bias, N, "bias")
     odt = out_dtype if out_dtype is not None else residual.dtype if residual is not None else torch.float16 if eight else x.dtype
-    if odt not in _ROW_TYPES:
+    ot = _ROW_TYPES.get(odt)
+    if ot is None:
         raise MpcError(f"linear: output type {odt} is not float32, float16 or bfloat16")
-    shape, rs = x.shape[:-1] + (N,), 0
+    shape, rs = (M, N) if len(xshape) == 2 else (*xshape[:-1], N), 0
     if residual is not None:
         if residual.shape != shape or residual.dtype != odt:
             raise MpcError(f"linear: residual {residual.dtype} {tuple(residual.shape)} does not match the output {odt} {tuple(shape)}")
         _, rs = _rows(residual, "residual")
-    out = torch.empty(shape, dtype=odt, device=x.device)
+    out = x.new_empty(shape, dtype=odt)
     if M == 0:
         return out
-    K = x.shape[-1]
-    desc = _lib.LinearDesc(_OPERAND_TYPES[x.dtype], _ROW_TYPES[odt], act, M, N, K, xs, ws, rs, N)
-    ws_bytes = _lib.load().mpc_linear_workspace_bytes(desc)
-    work = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    _call("linear", x.device, "mpc_linear_forward", desc, x.data_ptr(), _addr(x_scale), weight.data_ptr(), _addr(weight_scale), _addr(bias),
-          _addr(residual), _addr(work), ws_bytes, out.data_ptr(), flops=2.0 * M * N * K)
+    ctx = _lib.context_at(index)
+    desc = _lib.LinearDesc(t, ot, act, M, N, K, xs, ws, rs, N)
+    ws_bytes = ctx.lib.mpc_linear_workspace_bytes(desc)
+    work = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    args = (desc, x.data_ptr(), _addr(x_scale), weight.data_ptr(), _addr(weight_scale), _addr(bias), _addr(residual), _addr(work), ws_bytes,
+            out.data_ptr())
+    if PROFILER is None:
+        ctx.call("mpc_linear_forward", *args)
+    else:
+        with _timed("linear", flops=2.0 * M * N * K):
+            ctx.call("mpc_linear_forward", *args)
     return out
 
 
 def _balance_args(scores, scale, top_k, mask):
-    _same_gpu(scores, mask=mask)
-    if scores.dim() != 2 or scores.dtype not in _ROW_TYPES:
+    t = _ROW_TYPES.get(scores.dtype)
+    if t is None or scores.dim() != 2:
         raise MpcError(f"prior_balance: scores must be [rows, experts] float32, float16 or bfloat16 (got {scores.dtype} {tuple(scores.shape)})")
     T, E = scores.shape
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (T,) or not mask.is_contiguous()):
         raise MpcError(f"prior_balance: mask must be {T} contiguous bool values, got {mask.dtype} {tuple(mask.shape)}")
-    return (scores.data_ptr(), _ROW_TYPES[scores.dtype], T, E, scores.stride(0), scores.stride(1), scale, top_k, _addr(mask))
+    return (scores.data_ptr(), t, T, E, *scores.stride(), scale, top_k, _addr(mask))
 
 
 def prior_balance(scores: torch.Tensor, scale: float = 1.0, top_k: int = 1, mask: Optional[torch.Tensor] = None):
@@ -426,16 +440,19 @@ def prior_balance(scores: torch.Tensor, scale: float = 1.0, top_k: int = 1, mask
     -infinity) chooses its top_k best, ties to the lowest index.  loss = E * sum_e f_e P_e with f the share of the choices and
     P the mean of p: 1 for even use, up to E where one expert takes all; 0 without rows.  counts are the choices per
     expert.  Everything stays on the device; the order of the sums is fixed."""
+    index = _gpu_of(scores, mask)
     args = _balance_args(scores, scale, top_k, mask)
-    T, E = scores.shape
-    dev = scores.device
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    counts = torch.empty(E, dtype=torch.int32, device=dev)
-    n_rows = torch.empty(1, dtype=torch.int32, device=dev)
-    ws_bytes = _lib.load().mpc_prior_balance_workspace_bytes(T, E)
-    work = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _call("prior_balance", dev, "mpc_prior_balance", *args, work.data_ptr(), ws_bytes, loss.data_ptr(), counts.data_ptr(), n_rows.data_ptr(),
-          bytes=float(scores.numel()) * scores.element_size())
+    T, E = args[2:4]
+    ctx = _lib.context_at(index)
+    ws_bytes = ctx.lib.mpc_prior_balance_workspace_bytes(T, E)
+    loss, counts = scores.new_empty((), dtype=torch.float32), scores.new_empty(E, dtype=torch.int32)
+    n_rows, work = scores.new_empty(1, dtype=torch.int32), scores.new_empty(ws_bytes, dtype=torch.uint8)
+    args += (work.data_ptr(), ws_bytes, loss.data_ptr(), counts.data_ptr(), n_rows.data_ptr())
+    if PROFILER is None:
+        ctx.call("mpc_prior_balance", *args)
+    else:
+        with _timed("prior_balance", bytes=float(scores.numel()) * scores.element_size()):
+            ctx.call("mpc_prior_balance", *args)
     return loss, counts, n_rows
 
 
@@ -444,16 +461,20 @@ def prior_balance_grad(scores: torch.Tensor, counts: torch.Tensor, n_rows: torch
     """Gradient of prior_balance's loss in the scores, in their type and layout, times grad_out (fp32, one value on the
     device; None: 1).  counts and n_rows are what prior_balance returned for the same scores, scale, top_k and mask.  The
     choices count as constants, as usual for this loss; rows that do not count get zeros."""
-    _same_gpu(scores, counts=counts, n_rows=n_rows, grad_out=grad_out)
+    index = _gpu_of(scores, mask, counts, n_rows, grad_out)
     args = _balance_args(scores, scale, top_k, mask)
-    E = scores.shape[1]
-    for t, n, name in ((counts, E, "counts"), (n_rows, 1, "n_rows")):
+    for t, n, name in ((counts, args[3], "counts"), (n_rows, 1, "n_rows")):
         if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
             raise MpcError(f"prior_balance_grad: {name} must be {n} contiguous int32 values, got {t.dtype} {tuple(t.shape)}")
-    _vector(grad_out, 1, "grad_out")
+    if grad_out is not None:
+        _vector(grad_out, 1, "grad_out")
     grad = torch.empty_like(scores)
-    _call("prior_balance_grad", scores.device, "mpc_prior_balance_grad", *args, counts.data_ptr(), n_rows.data_ptr(), _addr(grad_out),
-          grad.data_ptr(), grad.stride(0), grad.stride(1), bytes=2.0 * scores.numel() * scores.element_size())
+    args += (counts.data_ptr(), n_rows.data_ptr(), _addr(grad_out), grad.data_ptr(), *grad.stride())
+    if PROFILER is None:
+        _lib.context_at(index).call("mpc_prior_balance_grad", *args)
+    else:
+        with _timed("prior_balance_grad", bytes=2.0 * scores.numel() * scores.element_size()):
+            _lib.context_at(index).call("mpc_prior_balance_grad", *args)
     return grad
 
 

@@ -180,7 +180,7 @@ def operands(seed, M, N, K, dtype):
 
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 1000, 200), (2, 33, 7), (3, 256, 1024), (7, 130, 4096), (15, 64, 129), (16, 512, 512), (17, 100, 333),
          (31, 320, 192), (33, 192, 320), (63, 65, 66), (64, 256, 256), (65, 1000, 128), (128, 128, 8192), (129, 127, 100), (200, 300, 400),
-         (257, 255, 513), (512, 1024, 256), (1000, 64, 1111), (1537, 1000, 144), (100, 3, 5000), (1, 5, 20000), (640, 640, 72)]
+         (257, 255, 513), (512, 1024, 256), (1000, 64, 1111), (1537, 1000, 144), (100, 3, 5000), (1, 5, 20000), (640, 640, 72), (500, 70, 5), (3000, 40, 1), (129, 1030, 15), (700, 200, 8)]
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
