@@ -231,8 +231,8 @@ __device__ __forceinline__ u32x4 row_end(u32x4 v, int sh) {
     return __builtin_bit_cast(u32x4, t);
 }
 
-// A tile's rows of an operand as a buffer: a row past the last gets an offset past the end, and such a load gives zeros.
-constexpr unsigned NO_ROW = 0x80000000u;
+// A tile's rows of an operand as a buffer that ends with the last row: a load for a row past it gives zeros or, where rows
+// overlap, values of other rows; neither reaches an output.
 constexpr int64_t TILE_BYTES = 1ll << 30;                         // most that a tile's rows may span (the host checks)
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 __device__ __forceinline__ rsrc_t tile_buffer(const char *base, int rows, int64_t stride, int64_t K) {
@@ -269,18 +269,14 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_t
     auto xkey = [](int r) { return r & 7; };
     auto wkey = [](int r) { return (r & 3) | (r >> 3 & 1) << 2; };
     const int p = tid & 7, r0 = tid >> 3;
-    unsigned xo[XP], wo[WP];
-#pragma unroll
-    for (int i = 0; i < XP; ++i) xo[i] = r0 + i * (NT / 8) < rows_x ? (unsigned)((r0 + i * (NT / 8)) * a.xs) : NO_ROW;
-#pragma unroll
-    for (int i = 0; i < WP; ++i) wo[i] = r0 + i * (NT / 8) < rows_w ? (unsigned)((r0 + i * (NT / 8)) * a.ws) : NO_ROW;
+    const unsigned xo = r0 * (unsigned)a.xs, wo = r0 * (unsigned)a.ws, xstep = (unsigned)a.xs * (NT / 8), wstep = (unsigned)a.ws * (NT / 8);
     u32x4 xr[DEPTH][XP], wr[DEPTH][WP];
     auto fetch = [&](int slot, int t) {                           // (past the row's end: its last piece)
         const int at = (t0 + t) * KT + p * 16, off = at < K - 16 ? at : K - 16;
 #pragma unroll
-        for (int i = 0; i < XP; ++i) xr[slot][i] = buffer_piece(xb, xo[i] + off);
+        for (int i = 0; i < XP; ++i) xr[slot][i] = buffer_piece(xb, xo + off + i * xstep);
 #pragma unroll
-        for (int i = 0; i < WP; ++i) wr[slot][i] = buffer_piece(wb, wo[i] + off);
+        for (int i = 0; i < WP; ++i) wr[slot][i] = buffer_piece(wb, wo + off + i * wstep);
     };
     auto stash = [&](int slot, int buf) {
         u32x4 *x = lds + buf * (BM + BN) * 8, *w = x + BM * 8;
@@ -482,22 +478,16 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     const int64_t m0 = (int64_t)tm * BIG, n0 = (int64_t)tn * BIG;
     const int rows_x = (int)(a.M - m0 < BIG ? a.M - m0 : BIG), rows_w = (int)(a.N - n0 < BIG ? a.N - n0 : BIG);
 
-    // A piece past K (a multiple of 16 bytes here) gets an offset past the end, like a row past the last.
-    constexpr unsigned NO_K = 0x40000000u;
     const rsrc_t xr = tile_buffer(a.x + m0 * a.xs, rows_x, a.xs, a.K), wr = tile_buffer(a.w + n0 * a.ws, rows_w, a.ws, a.K);
     const int p = tid & 7, r0 = tid >> 3;
-    unsigned xo[8], wo[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = r0 + 32 * i;
-        xo[i] = r < rows_x ? (unsigned)(r * a.xs) + p * 16 : NO_ROW;
-        wo[i] = r < rows_w ? (unsigned)(r * a.ws) + p * 16 : NO_ROW;
-    }
+    const unsigned xo = r0 * (unsigned)a.xs + p * 16, wo = r0 * (unsigned)a.ws + p * 16;
+    const unsigned xstep = 32 * (unsigned)a.xs, wstep = 32 * (unsigned)a.ws;
     u32x4 xg[8], wg[8];
     const int K = (int)a.K;
-    auto k_offset = [&](int k) { return k + p * 16 < K ? (unsigned)k : NO_K; };
-    auto fetch_x = [&](int i, unsigned ko) { xg[i] = buffer_piece(xr, xo[i] + ko); };
-    auto fetch_w = [&](int i, unsigned ko) { wg[i] = buffer_piece(wr, wo[i] + ko); };
+    // (a piece past K, a multiple of 16 bytes here, gets an offset past the end: zeros)
+    auto k_offset = [&](int k) { return k + p * 16 < K ? (unsigned)k : 0x80000000u; };
+    auto fetch_x = [&](int i, unsigned ko) { xg[i] = buffer_piece(xr, xo + ko + i * xstep); };
+    auto fetch_w = [&](int i, unsigned ko) { wg[i] = buffer_piece(wr, wo + ko + i * wstep); };
     // LDS slots, as in the kernel above: piece p of row r at p ^ key(r); rows of w are read interleaved, so its
     // key takes bit 3 of the row.  [x buffer 0][x buffer 1][w buffer 0][w buffer 1], each 256 rows of 8 pieces.
     u32x4 *const xdst = lds + r0 * 8 + (p ^ (r0 & 7));
@@ -725,8 +715,10 @@ Plan plan_for(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {     // 
     if (big >= 256 && K >= 2048) return {PLAN_BIG, 1};
     if (middle >= 200) return {PLAN_MIDDLE, 1};
     const int64_t small = mpc_cdiv(M, 64) * mpc_cdiv(N, 64), k_tiles = mpc_cdiv(K, KT);
+    // A k-tile takes 0.25 us with a workgroup per CU, 0.4 with two; joining the splits takes 8 us and more.  (1537 x 1000 x 1024:
+    // 10.7 us in one, 20 in two; 64 x 8192 x 8192: 44 in one, 28 in four.)
     int splits = 1;
-    while (splits < 16 && small * splits * 2 <= 1024 && k_tiles / (splits * 2) >= 8) splits *= 2;
+    while (splits < 16 && small * splits * 2 <= 512 && k_tiles / (splits * 2) >= 16) splits *= 2;
     return {PLAN_SMALL, splits};
 }
 
