@@ -61,10 +61,24 @@ __device__ __forceinline__ void activate(float (&v)[V], int act) {
     }
 }
 
+// One of the rows kept in registers, whose index is known only at run time: a copy for each (the empty asm keeps the copies
+// from being merged into one through a pointer, which would put the rows into memory).
+template <int ROWS, int P, typename Vec, int M = 0>
+__device__ __forceinline__ void take_row(const Vec (&rows)[ROWS][P], int m, Vec (&out)[P]) {
+    if constexpr (M + 1 < ROWS) {
+        if (m != M) return take_row<ROWS, P, Vec, M + 1>(rows, m, out);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        u32x4 t = __builtin_bit_cast(u32x4, rows[M][i]);
+        asm("" : "+v"(t));
+        out[i] = __builtin_bit_cast(Vec, t);
+    }
+}
+
 // The rows of a lane: row0 + 16 m; its V columns are V / 8 runs of 8, n + 32 t .. n + 32 t + 7: the four lanes of a row then
 // write 64 consecutive bytes at a time.  take(m, v) gives the sums.  One rolled loop (the sums have fixed
-// registers, so take is a switch over copies): unrolled it would be tens of KB of code.  The next row's residual is on its way while
-// a row is worked on.
+// registers, so take is a switch over copies): unrolled it would be tens of KB of code.
 template <typename T, int MF, int V, typename Take>
 __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, int64_t n, Take take) {
     constexpr int PER = 16 / sizeof(T), P = V / PER;
@@ -77,25 +91,31 @@ __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, i
         b[i] = a.bias && col(i) < a.N ? a.bias[col(i)] : 0.0f;
         s[i] = a.sw && col(i) < a.N ? a.sw[col(i)] : 1.0f;
     }
-    vec_t next[P];
-    auto fetch = [&](int64_t row) {
+    // the residual's rows: up to four at once for 16-bit types, the next one while a row is worked on for fp32
+    constexpr int KEPT = sizeof(T) == 2 ? (MF < 4 ? MF : 4) : 1;
+    vec_t ahead[KEPT][P];
+    auto fetch = [&](int m, vec_t (&to)[P]) {
+        const int64_t row = row0 + 16 * m < a.M ? row0 + 16 * m : a.M - 1;
         const T *r = (const T *)(a.res + row * a.rs);
 #pragma unroll
-        for (int i = 0; i < P; ++i) next[i] = *(const vec_t *)(r + col(i * PER));
+        for (int i = 0; i < P; ++i) to[i] = *(const vec_t *)(r + col(i * PER));
     };
-    if (vec_res && row0 < a.M) fetch(row0);
+    if (vec_res && KEPT == 1) fetch(0, ahead[0]);
 #pragma unroll 1
     for (int m = 0; m < MF; ++m) {
         const int64_t row = row0 + 16 * m;
+        if (vec_res && KEPT > 1 && m % KEPT == 0) {
+#pragma unroll
+            for (int i = 0; i < KEPT; ++i) fetch(m + i, ahead[i]);
+        }
         float v[V];
         take(m, v);
-        if (row >= a.M) break;
         vec_t res[P];
         if (vec_res) {
-#pragma unroll
-            for (int i = 0; i < P; ++i) res[i] = next[i];
-            if (m + 1 < MF && row + 16 < a.M) fetch(row + 16);
+            take_row<KEPT, P>(ahead, m % KEPT, res);
+            if (KEPT == 1 && m + 1 < MF) fetch(m + 1, ahead[0]);
         }
+        if (row >= a.M) break;
         if (a.sx) {
             const float sx = a.sx[row];
 #pragma unroll
@@ -532,6 +552,15 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     };
     using Lo = std::integral_constant<int, 0>;
     using Hi = std::integral_constant<int, 1>;
+    // e4m3: the lines of the tile 2 further on are brought to the L2, by loads of a word each that nothing uses: 8 x 4 workgroups
+    // of an XCD share their operands and would all wait for a line that none had yet (235 -> 225 us for 8192 x 8192 x 4096;
+    // 16-bit products, which meet the power limit first, gain nothing).  Each workgroup takes its share of its tile's rows.
+    constexpr int AHEAD = 2;
+    const rsrc_t lr = wave & 1 ? wr : xr;
+    const int half = wave >> 1;
+    const unsigned lo = wave & 1 ? (unsigned)(8 * ((lane & 15) + 16 * half) + (tm & 7)) * (unsigned)a.ws
+                                 : (unsigned)(4 * ((lane & 31) + 32 * half) + (tn & 3)) * (unsigned)a.xs;
+    unsigned line = 0;
     Half x0, x1, w0, w1;
     // One k-tile from buffer `buf`; x0 and the first w half (wa) are in registers, the pieces of the next tile in xg, wg or on
     // their way.  k2: where the tile after the next begins (past the end: zeros are fetched, and never read).  The other
@@ -541,6 +570,10 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     auto tile = [&](int buf, int k2, Half &wa, Half &wb, auto ha, auto hb) {
         constexpr int WB = decltype(hb)::value;
         const unsigned ko = k_offset(k2), ko3 = k_offset(k2 + KT);
+        if constexpr (TYPE == MPC_TYPE_E4M3) {
+            asm volatile("" ::"v"(line));                     // (the line asked for a tile ago; older than pieces waited for below)
+            line = __builtin_amdgcn_raw_buffer_load_b32(lr, lo + (k2 + AHEAD * KT < K ? (unsigned)(k2 + AHEAD * KT) : 0x80000000u), 0, 0);
+        }
         multiply(wa, x0, ha, Lo{}, [&](int i) {
             if (i < 4) read_w(wb, 2 * i, buf, WB), read_w(wb, 2 * i + 1, buf, WB);
             if (i % 2 == 0) move(4 + i / 2, buf ^ 1, ko);
