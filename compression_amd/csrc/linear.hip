@@ -745,8 +745,12 @@ Plan plan_for(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {     // 
     // (rows shorter than a piece, or so far apart that a tile's do not fit a buffer: the kernel that addresses each by itself)
     if (M <= 32 || K < 16 || BIG * xs + K > TILE_BYTES || BIG * ws + K > TILE_BYTES) return {PLAN_ROWS, 1};
     const int64_t big = mpc_cdiv(M, BIG) * mpc_cdiv(N, BIG), middle = mpc_cdiv(M, 128) * mpc_cdiv(N, 128);
-    if (big >= 256 && K >= 2048) return {PLAN_BIG, 1};
-    if (middle >= 200) return {PLAN_MIDDLE, 1};
+    // The large tile needs most CUs busy and some k-tiles to pay for its prologue and epilogue (128 x 128 tiles against it, bf16
+    // with bias and gelu: 3584 x 4096 x 4096 137 us : 105; 2048 x 4096 x 4096 77 : 99; 4096 x 4096 x 1024 46 : 47; 8192 x 8192 x
+    // 512 114 : 119).  64 x 64 tiles take over where 128 x 128 ones are fewer than the CUs (768 x 4096 x 4096 44 : 39; 512 x 4096 x
+    // 4096 32 : 39).
+    if (big >= 192 && K >= 2048) return {PLAN_BIG, 1};
+    if (middle >= 176) return {PLAN_MIDDLE, 1};
     const int64_t small = mpc_cdiv(M, 64) * mpc_cdiv(N, 64), k_tiles = mpc_cdiv(K, KT);
     // A k-tile takes 0.25 us with a workgroup per CU, 0.4 with two; joining the splits takes 8 us and more.  (1537 x 1000 x 1024:
     // 10.7 us in one, 20 in two; 64 x 8192 x 8192: 44 in one, 28 in four.)
@@ -761,7 +765,9 @@ int launch(mpc_ctx *ctx, const LinearArgs &a) {
     if (plan.kind == PLAN_ROWS) return a.M <= 16 ? launch_rows<TYPE, 1>(ctx, a) : launch_rows<TYPE, 2>(ctx, a);
     if (plan.kind == PLAN_BIG && big_possible(a)) return launch_big<TYPE>(ctx, a);
     if (plan.kind == PLAN_SMALL) return launch_tiles<TYPE, 64, 64, 32, 32, 4, 3>(ctx, a, plan.splits);
-    return launch_tiles<TYPE, 128, 128, 64, 64, 2, 2>(ctx, a, 1);
+    // 8 waves of 64 x 32, two workgroups a CU: the second's products run beside the first's epilogue.  (36864 x 256 -> 1024 with
+    // gelu: 50 us; 4 waves of 64 x 64, with one or two tiles ahead: 53; 128 x 64 tiles: 52; 256 x 128: 63.)
+    return launch_tiles<TYPE, 128, 128, 64, 32, 1, 4>(ctx, a, 1);
 }
 
 bool linear_desc_ok(const mpc_linear_desc &d) {

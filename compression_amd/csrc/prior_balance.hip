@@ -9,6 +9,8 @@
 // prior) go through an LDS tile, read and, for the gradient, written along the rows.
 #include "row_ops.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int PB_MAX_EXPERTS = 1024;
@@ -37,9 +39,10 @@ __device__ __forceinline__ int dpp(int v) {
 }
 
 // op over the lanes of a group; every lane gets the result.  Lane i of a quad with i ^ 1, with i ^ 2, then the mirror
-// images of eight and of sixteen lanes.
-template <typename T, typename Op>
+// images of eight and of sixteen lanes.  LOG2: of the group's size, or -1 if that is known only at run time (`group`).
+template <int LOG2, typename T, typename Op>
 __device__ __forceinline__ T group_reduce(T v, int group, Op op) {
+    if constexpr (LOG2 >= 0) group = 1 << LOG2;
     if (group > 1) v = op(v, dpp<0xB1>(v));
     if (group > 2) v = op(v, dpp<0x4E>(v));
     if (group > 4) v = op(v, dpp<0x141>(v));
@@ -115,18 +118,18 @@ __device__ __forceinline__ void staged_values(const Row &a, const float *tile_ro
 }
 
 // v -> p = e * inv.  Returns whether the row counts (inv = 0 if not).  Changes v only in rows without anything above -inf.
-template <int EPL>
+template <int LOG2, int EPL>
 __device__ __forceinline__ bool softmax(const Row &a, bool keep, float (&v)[EPL], float (&e)[EPL], float &top, float &inv) {
     const float slope = fabsf(a.scale) * 1.44269504f;
     top = v[0];
 #pragma unroll
     for (int j = 1; j < EPL; ++j) top = fmaxf(top, v[j]);
-    top = group_reduce(top, a.group, Max());
+    top = group_reduce<LOG2>(top, a.group, Max());
     if (__any(keep && top == -INFINITY)) {                    // rows of -inf (and NaN): rare
         int nan = 0;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) nan |= v[j] != v[j];
-        nan = group_reduce(nan, a.group, Or());
+        nan = group_reduce<LOG2>(nan, a.group, Or());
         if (top == -INFINITY && !nan) {
             keep = false;
             top = 0.0f;
@@ -138,7 +141,7 @@ __device__ __forceinline__ bool softmax(const Row &a, bool keep, float (&v)[EPL]
         e[j] = __builtin_amdgcn_exp2f((v[j] - top) * slope);
         sum += e[j];
     }
-    sum = group_reduce(sum, a.group, Add());
+    sum = group_reduce<LOG2>(sum, a.group, Add());
     inv = keep ? __builtin_amdgcn_rcpf(sum) : 0.0f;
     return keep;
 }
@@ -197,8 +200,9 @@ __device__ __forceinline__ void stage(const Row &a, int64_t first, float *tile) 
 }
 
 // words of a block in the workspace: sum of p (float) [experts], choices (int) [experts], rows (int)
-template <typename T, int EPL, bool STAGED>
+template <typename T, int EPL, int LOG2, bool STAGED>
 __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_kernel(Row a, float *__restrict__ ws) {
+    if constexpr (LOG2 >= 0) a.group = 1 << LOG2, a.group_log2 = LOG2;
     extern __shared__ float lds[];                            // [experts] choices | sums of the waves, or the tile
     __shared__ int rsum[PB_MAX_THREADS / 64];
     int *hist = (int *)lds;
@@ -214,7 +218,7 @@ __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_kernel(Row a, fl
 
     auto one = [&](bool keep, float (&v)[EPL]) {
         float e[EPL], top, inv;
-        keep = softmax<EPL>(a, keep, v, e, top, inv);
+        keep = softmax<LOG2, EPL>(a, keep, v, e, top, inv);
 #pragma unroll
         for (int j = 0; j < EPL; ++j) acc[j] = fmaf(e[j], inv, acc[j]);          // (rows that do not count: inv = 0, e finite)
         n += (int)__popcll(__ballot(keep && e0 == 0));
@@ -224,12 +228,12 @@ __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_kernel(Row a, fl
                 best = v[0];
 #pragma unroll
                 for (int j = 1; j < EPL; ++j) best = fmaxf(best, v[j]);
-                best = group_reduce(best, a.group, Max());
+                best = group_reduce<LOG2>(best, a.group, Max());
             }
             int at_e = PB_MAX_EXPERTS;
 #pragma unroll
             for (int j = EPL - 1; j >= 0; --j) at_e = v[j] == best ? e0 + j : at_e;
-            at_e = group_reduce(at_e, a.group, Min());
+            at_e = group_reduce<LOG2>(at_e, a.group, Min());
             if (keep && best > -INFINITY && e0 == 0) atomicAdd(&hist[at_e], 1);
             if (k + 1 < a.top_k) {
 #pragma unroll
@@ -334,11 +338,12 @@ __global__ __launch_bounds__(1024) void prior_balance_join_kernel(const float *_
     }
 }
 
-template <typename T, int EPL, bool STAGED>
+template <typename T, int EPL, int LOG2, bool STAGED>
 __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_grad_kernel(Row a, const int32_t *__restrict__ counts,
                                                                             const int32_t *__restrict__ n_rows,
                                                                             const float *__restrict__ grad_out, T *__restrict__ grad,
                                                                             int64_t grs, int64_t ges) {
+    if constexpr (LOG2 >= 0) a.group = 1 << LOG2, a.group_log2 = LOG2;
     extern __shared__ float tile[];
     constexpr int W = 16 / sizeof(T);
     typedef T vec __attribute__((ext_vector_type(W)));
@@ -355,14 +360,14 @@ __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_grad_kernel(Row 
 
     auto one = [&](int64_t row, bool in, bool keep, float (&v)[EPL], float *tile_row) {
         float e[EPL], top, inv;
-        keep = softmax<EPL>(a, keep, v, e, top, inv);
+        keep = softmax<LOG2, EPL>(a, keep, v, e, top, inv);
         float d = 0.0f;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
             e[j] *= inv;                                      // (rows that do not count: inv = 0, e finite)
             d = fmaf(e[j], f[j], d);
         }
-        d = group_reduce(d, a.group, Add());
+        d = group_reduce<LOG2>(d, a.group, Add());
         const float gk = keep ? g : 0.0f;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) e[j] *= gk * (f[j] - d);
@@ -479,6 +484,20 @@ Shape shape(Row &a, bool staged) {
     return s;
 }
 
+// f(the group's log2 as a constant): with it the reductions are straight code (1M x 64 bf16, top 2: forward 77 -> 71 us)
+template <typename F>
+void by_group(int log2, F f) {
+    switch (log2) {
+        case 0: return f(std::integral_constant<int, 0>());
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 3: return f(std::integral_constant<int, 3>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 5: return f(std::integral_constant<int, 5>());
+        default: return f(std::integral_constant<int, 6>());
+    }
+}
+
 template <typename T>
 int forward(mpc_ctx *ctx, Row a, float *ws, float *loss, int32_t *counts, int32_t *n_rows) {
     const bool staged = a.expert_stride != 1 && a.experts > 1;
@@ -488,10 +507,10 @@ int forward(mpc_ctx *ctx, Row a, float *ws, float *loss, int32_t *counts, int32_
     if (sums < s.tile_bytes) sums = s.tile_bytes;
     const size_t lds = a.experts * sizeof(int) + sums;
     const dim3 grid(blocks), block(s.threads);
-    if (s.epl == 8 && !staged) prior_balance_kernel<T, 8, false><<<grid, block, lds, ctx->stream>>>(a, ws);
-    if (s.epl == 8 && staged) prior_balance_kernel<T, 8, true><<<grid, block, lds, ctx->stream>>>(a, ws);
-    if (s.epl == 16 && !staged) prior_balance_kernel<T, 16, false><<<grid, block, lds, ctx->stream>>>(a, ws);
-    if (s.epl == 16 && staged) prior_balance_kernel<T, 16, true><<<grid, block, lds, ctx->stream>>>(a, ws);
+    auto run = [&](auto kernel) { kernel<<<grid, block, lds, ctx->stream>>>(a, ws); };
+    if (staged) s.epl == 8 ? run(prior_balance_kernel<T, 8, -1, true>) : run(prior_balance_kernel<T, 16, -1, true>);
+    else if (s.epl == 16) run(prior_balance_kernel<T, 16, 6, false>);
+    else by_group(a.group_log2, [&](auto log2) { run(prior_balance_kernel<T, 8, decltype(log2)::value, false>); });
     MPC_CHECK_LAUNCH(ctx, "prior_balance");
     prior_balance_join_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(ws, blocks, a.experts, 1024 / a.experts, a.top_k, loss, counts, n_rows);
     MPC_CHECK_LAUNCH(ctx, "prior_balance_join");
@@ -504,10 +523,10 @@ int backward(mpc_ctx *ctx, Row a, const int32_t *counts, const int32_t *n_rows, 
     const Shape s = shape(a, staged);
     const dim3 grid((unsigned)(s.passes > 1024 ? 1024 : s.passes)), block(s.threads);
     T *o = (T *)grad;
-    if (s.epl == 8 && !staged) prior_balance_grad_kernel<T, 8, false><<<grid, block, 0, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
-    if (s.epl == 8 && staged) prior_balance_grad_kernel<T, 8, true><<<grid, block, s.tile_bytes, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
-    if (s.epl == 16 && !staged) prior_balance_grad_kernel<T, 16, false><<<grid, block, 0, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
-    if (s.epl == 16 && staged) prior_balance_grad_kernel<T, 16, true><<<grid, block, s.tile_bytes, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges);
+    auto run = [&](auto kernel) { kernel<<<grid, block, staged ? s.tile_bytes : 0, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges); };
+    if (staged) s.epl == 8 ? run(prior_balance_grad_kernel<T, 8, -1, true>) : run(prior_balance_grad_kernel<T, 16, -1, true>);
+    else if (s.epl == 16) run(prior_balance_grad_kernel<T, 16, 6, false>);
+    else by_group(a.group_log2, [&](auto log2) { run(prior_balance_grad_kernel<T, 8, decltype(log2)::value, false>); });
     MPC_CHECK_LAUNCH(ctx, "prior_balance_grad");
     return MPC_OK;
 }
