@@ -15,6 +15,7 @@ namespace {
 
 constexpr int PB_MAX_EXPERTS = 1024;
 constexpr int PB_MAX_THREADS = 512;
+constexpr int PB_WIDE_THREADS = 1024;   // forward kernel of consecutive experts (1M x 64 bf16, top 2: 56 us against 61 with 512)
 constexpr int PB_MAX_BLOCKS = 512;
 
 struct Row {
@@ -201,10 +202,10 @@ __device__ __forceinline__ void stage(const Row &a, int64_t first, float *tile) 
 
 // words of a block in the workspace: sum of p (float) [experts], choices (int) [experts], rows (int)
 template <typename T, int EPL, int LOG2, bool STAGED>
-__global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_kernel(Row a, float *__restrict__ ws) {
+__global__ __launch_bounds__(STAGED ? PB_MAX_THREADS : PB_WIDE_THREADS) void prior_balance_kernel(Row a, float *__restrict__ ws) {
     if constexpr (LOG2 >= 0) a.group = 1 << LOG2, a.group_log2 = LOG2;
     extern __shared__ float lds[];                            // [experts] choices | sums of the waves, or the tile
-    __shared__ int rsum[PB_MAX_THREADS / 64];
+    __shared__ int rsum[PB_WIDE_THREADS / 64];
     int *hist = (int *)lds;
     float *tile = lds + a.experts;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
@@ -259,10 +260,11 @@ __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_kernel(Row a, fl
     } else {
         const int64_t step = (int64_t)gridDim.x * per_block;
         int64_t first = (int64_t)blockIdx.x * per_block + wave * per_wave;
+        const int mine = lane >> a.group_log2;
         Raw<T, EPL> now, next;
-        if (first < a.rows) now.fetch(a, first + (lane >> a.group_log2), e0);
+        if (a.rows > 0) now.fetch(a, first + mine, e0);       // (with no row at all there is none to read in a missing one's place)
         for (; first < a.rows; first += step) {               // the next rows are on their way while these are worked on
-            if (first + step < a.rows) next.fetch(a, first + step + (lane >> a.group_log2), e0);
+            next.fetch(a, first + step + mine, e0);
             float v[EPL];
             now.values(a, v);
             one(now.keep, v);
@@ -309,7 +311,7 @@ __global__ __launch_bounds__(1024) void prior_balance_join_kernel(const float *_
     double p = 0.0;
     int c = 0;
     if (slice < slices) {
-#pragma unroll 4
+#pragma unroll 8
         for (int b = slice; b < blocks; b += slices) {
             p += (double)ws[(int64_t)b * words + e];
             c += ((const int *)ws)[(int64_t)b * words + experts + e];
@@ -459,7 +461,7 @@ struct Shape {
 };
 
 // Lanes per row, rows per tile, threads per block.  Few rows: small blocks, so that more CUs take part.
-Shape shape(Row &a, bool staged) {
+Shape shape(Row &a, bool staged, int most) {
     Shape s{};
     s.epl = a.experts > 8 * 64 ? 16 : 8;
     a.group = 1, a.group_log2 = 0;
@@ -477,14 +479,14 @@ Shape shape(Row &a, bool staged) {
         s.tile_bytes = (size_t)r * (a.experts + 1) * sizeof(float);
         per_block = r;
     } else {
-        s.threads = few ? 128 : PB_MAX_THREADS;
+        s.threads = few ? 128 : most;
         per_block = s.threads / a.group;
     }
     s.passes = a.rows > 0 ? mpc_cdiv(a.rows, per_block) : 1;
     return s;
 }
 
-// f(the group's log2 as a constant): with it the reductions are straight code (1M x 64 bf16, top 2: forward 77 -> 71 us)
+// f(the group's log2 as a constant): with it the reductions are straight code (1M x 64 bf16, top 2: forward 77 -> 71 us, gradient 78 -> 51)
 template <typename F>
 void by_group(int log2, F f) {
     switch (log2) {
@@ -501,7 +503,7 @@ void by_group(int log2, F f) {
 template <typename T>
 int forward(mpc_ctx *ctx, Row a, float *ws, float *loss, int32_t *counts, int32_t *n_rows) {
     const bool staged = a.expert_stride != 1 && a.experts > 1;
-    const Shape s = shape(a, staged);
+    const Shape s = shape(a, staged, PB_WIDE_THREADS);
     const int blocks = (int)(s.passes > PB_MAX_BLOCKS ? PB_MAX_BLOCKS : s.passes);
     size_t sums = (size_t)(s.threads / 64) * a.group * s.epl * sizeof(float);
     if (sums < s.tile_bytes) sums = s.tile_bytes;
@@ -520,7 +522,7 @@ int forward(mpc_ctx *ctx, Row a, float *ws, float *loss, int32_t *counts, int32_
 template <typename T>
 int backward(mpc_ctx *ctx, Row a, const int32_t *counts, const int32_t *n_rows, const float *grad_out, void *grad, int64_t grs, int64_t ges) {
     const bool staged = a.expert_stride != 1 && a.experts > 1;
-    const Shape s = shape(a, staged);
+    const Shape s = shape(a, staged, PB_MAX_THREADS);
     const dim3 grid((unsigned)(s.passes > 1024 ? 1024 : s.passes)), block(s.threads);
     T *o = (T *)grad;
     auto run = [&](auto kernel) { kernel<<<grid, block, staged ? s.tile_bytes : 0, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges); };

@@ -1,6 +1,11 @@
-"""The row operators' refusals (no kernel is launched: every call is turned down before it reaches the GPU) and the host's
-view of strided rows."""
+"""The row operators without a GPU: refusals (every call is turned down before it reaches the GPU), the host's
+view of strided rows, and what the built code of the large product looks like."""
 import ctypes
+import os
+import re
+import shutil
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -55,3 +60,76 @@ def test_entry_points_refuse_a_null_context():
     assert lib.mpc_rms_norm(None, None, 0, None, 0, None, 1, 1, 0.0, 0, None, None, 0, None) == -1
     assert lib.mpc_prior_balance(None, None, 0, 1, 1, 1, 1, 1.0, 1, None, None, 0, None, None, None) == -1
     assert lib.mpc_prior_balance_grad(None, None, 0, 1, 1, 1, 1, 1.0, 1, None, None, None, None, None, 1, 1) == -1
+
+
+# ---- the large product's matrix instructions, which the compiler does not see as such (inline asm) -------------------------
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+LLVM = "/opt/rocm/lib/llvm/bin"
+
+
+def _registers(text):
+    out = set()
+    for kind, lo, hi in re.findall(r"\b([va])\[(\d+):(\d+)\]", text):
+        out |= {(kind, i) for i in range(int(lo), int(hi) + 1)}
+    return out | {(kind, int(i)) for kind, i in re.findall(r"\b([va])(\d+)\b", text)}
+
+
+@pytest.fixture(scope="module")
+def big_kernels(tmp_path_factory):
+    """{symbol: instructions} of linear_big_kernel in the built library."""
+    lib = os.path.join(REPO, "compression_amd", "libmpc.so")
+    if not os.path.exists(lib) or not os.path.exists(os.path.join(LLVM, "llvm-objdump")):
+        pytest.skip("needs the ROCm LLVM tools and a built libmpc.so")
+    tmp = str(tmp_path_factory.mktemp("code"))
+    copy = os.path.join(tmp, "lib.so")
+    shutil.copy(lib, copy)
+    subprocess.run([os.path.join(LLVM, "llvm-objdump"), "--offloading", copy], cwd=tmp, check=True, capture_output=True)
+    out = {}
+    for name in sorted(os.listdir(tmp)):
+        if "amdgcn" not in name:
+            continue
+        path = os.path.join(tmp, name)
+        symbols = subprocess.run([os.path.join(LLVM, "llvm-readelf"), "--symbols", "--wide", path], capture_output=True, text=True, check=True).stdout
+        for symbol in sorted(set(re.findall(r"\S*linear_big_kernel\S*", symbols))):
+            if symbol.endswith(".kd"):
+                continue
+            text = subprocess.run([os.path.join(LLVM, "llvm-objdump"), "-d", "--no-show-raw-insn", "--no-leading-addr",
+                                   "--disassemble-symbols=" + symbol, path], capture_output=True, text=True, check=True).stdout
+            lines = [re.sub(r"\s*//.*", "", x).strip() for x in text.split("\n")]
+            out[symbol] = [x for x in lines if re.match(r"(v|s|ds|buffer|global|scratch)_\w+", x)]
+    return out
+
+
+def test_large_product_waits_for_its_matrix_instructions(big_kernels):
+    """What the compiler would see to, had it known them: no vector instruction writes an operand within two instructions ahead of
+    a matrix instruction that reads it, and none reads sums within 18 wait states of the last matrix instruction."""
+    assert len(big_kernels) == 3
+    for symbol, code in big_kernels.items():
+        matrix = [i for i, x in enumerate(code) if x.startswith("v_mfma")]
+        assert len(matrix) >= 128, symbol
+        for i in matrix:
+            used = _registers(code[i])
+            for x in code[max(0, i - 2):i]:
+                if x.startswith("v_") and not x.startswith(("v_mfma", "v_cmp", "v_readfirstlane")):
+                    assert not _registers(x.split(None, 1)[1].split(",")[0]) & used, (symbol, x, code[i])
+        waited = 0
+        for x in code[matrix[-1] + 1:]:
+            if waited >= 18:
+                break
+            if x.startswith("s_nop"):
+                waited += int(x.split()[1]) + 1
+            else:
+                waited += 1
+                assert not (x.startswith("v_") and any(kind == "a" for kind, _ in _registers(x))), (symbol, x)
+        assert any(x.startswith("s_nop 15") for x in code[matrix[-1]:matrix[-1] + 12]), symbol
+
+
+def test_large_product_keeps_its_sums_in_registers():
+    sys.path.insert(0, os.path.join(REPO, "tools"))
+    import kernel_registers
+    if not os.path.exists(os.path.join(REPO, "compression_amd", "libmpc.so")) or not os.path.exists(os.path.join(LLVM, "llvm-objdump")):
+        pytest.skip("needs the ROCm LLVM tools and a built libmpc.so")
+    big = {n: k for n, k in kernel_registers.kernels().items() if "linear_big_kernel" in n}
+    assert len(big) == 3
+    for name, k in big.items():
+        assert k["agpr"] == 256 and k["vgpr"] + k["agpr"] <= 512 and k["scratch"] <= 64, (name, k)

@@ -15,7 +15,8 @@ REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def kernels(library=None):
-    """-> {kernel name (demangled where c++filt is installed): {"vgpr": n, "agpr": n, "sgpr": n, "lds": bytes, "scratch": bytes}}"""
+    """-> {kernel name (demangled where c++filt is installed): {"vgpr": n, "agpr": n, "sgpr": n, "lds": bytes, "scratch": bytes}},
+    a SIMD lane's 512 registers holding vgpr + agpr of every wave"""
     library = library or os.path.join(REPO, "compression_amd", "libmpc.so")
     out = {}
     with tempfile.TemporaryDirectory() as tmp:
@@ -31,7 +32,9 @@ def kernels(library=None):
                 fields = dict(re.findall(r"\.(\w+):\s+(\S+)", ".agpr_count:" + block.split("\n  - .agpr_count:")[0]))
                 if "name" not in fields or "vgpr_count" not in fields:
                     continue
-                out[fields["name"]] = dict(vgpr=int(fields["vgpr_count"]), agpr=int(fields["agpr_count"]), sgpr=int(fields["sgpr_count"]),
+                # (gfx90a and later: .vgpr_count is the sum of both kinds, the accumulation registers behind the others)
+                agpr = int(fields["agpr_count"])
+                out[fields["name"]] = dict(vgpr=int(fields["vgpr_count"]) - agpr, agpr=agpr, sgpr=int(fields["sgpr_count"]),
                                            lds=int(fields.get("group_segment_fixed_size", 0)),
                                            scratch=int(fields.get("private_segment_fixed_size", 0)))
     if out:
