@@ -26,6 +26,8 @@ void mpc_ctx_scratch_release(mpc_ctx *ctx);
 // Looks up this device's instance of the static scratch of mpc_rans_decode_noalloc (rans.hip); the context's device
 // must be current.  Called by mpc_create.
 int mpc_rans_static_init(mpc_ctx *ctx);
+// Sets what the kernels of linear.hip need set once per device.  Called by mpc_create, with the context's device current.
+int mpc_linear_init(mpc_ctx *ctx);
 
 #define MPC_FAIL(ctx, code, ...)                                   \
     do {                                                           \

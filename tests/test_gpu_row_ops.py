@@ -198,7 +198,8 @@ def test_linear(dtype, M, N, K):
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("M,N,K", SIZES + [(700, 900, 2000), (3, 4096, 4096), (5000, 260, 1030), (4200, 4104, 512), (4097, 4160, 16), (66000, 250, 80),
-                                           (4352, 4096, 144), (200, 70000, 208), (5000, 4000, 1152)])
+                                           (4352, 4096, 144), (200, 70000, 208), (5000, 4000, 1152), (4200, 4104, 2064), (3600, 3600, 2048),
+                                           (33, 500, 12345), (2000, 1500, 1999)])
 def test_linear_whole_numbers_exactly(dtype, M, N, K):
     """Small whole operands: every product and sum is a whole number below 2^24, exact in fp32 and on the 8-bit
     instructions' grid, so one value of k too many, too few or in the wrong place shows."""
@@ -215,7 +216,7 @@ def test_linear_whole_numbers_exactly(dtype, M, N, K):
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("M,N,K", [(2100, 2050, 520), (4096, 1024, 256), (8200, 256, 1024), (3000, 4100, 136), (9, 4096, 4096), (300, 4096, 2048),
-                                   (36864, 64, 256), (2048, 2048, 2048), (5000, 1030, 1040), (4200, 4104, 512), (8192, 2048, 272)])
+                                   (36864, 64, 256), (2048, 2048, 2048), (5000, 1030, 1040), (4200, 4104, 512), (8192, 2048, 272), (4200, 4104, 2064), (3600, 3700, 2048)])
 def test_linear_large(dtype, M, N, K):
     from compression_amd import ops
     x, w, sx, sw = operands(M + N + K, M, N, K, dtype)
@@ -270,7 +271,28 @@ def test_linear_special_values_stay_where_they_are(dtype, M, K):
     assert bool(torch.isnan(got[:, N - 1]).all()) and torch.equal(got[:, :N - 1], clean[:, :N - 1])
 
 
-@pytest.mark.parametrize("M,N,K,dtype", [(1, 100, 256, F16), (20, 70, 4096, BF16), (130, 129, 64, E4M3), (300, 512, 128, BF16)])
+@pytest.mark.parametrize("dtype,K", [(BF16, 1040), (E4M3, 2064)])
+def test_large_tiles_keep_to_their_rows(dtype, K):
+    """The same at the size of the large tiles: NaN behind the rows' ends, behind the last rows, and in one row of each operand."""
+    from compression_amd import ops
+    M, N, pad = 3700, 3650, 16 if dtype == E4M3 else 8
+    x, w, sx, sw = operands(16, M, N, K, dtype)
+    clean = ops.linear(x, w, None, 0, None, sx, sw, F32)
+    px = torch.full((M + 300, K + pad), float("nan"), device=DEV).to(dtype)
+    pw = torch.full((N + 300, K + pad), float("nan"), device=DEV).to(dtype)
+    px[:M, :K], pw[:N, :K] = x, w
+    assert torch.equal(ops.linear(px[:M, :K], pw[:N, :K], None, 0, None, sx, sw, F32), clean)
+    px[M - 1, K - 1] = float("nan")
+    got = ops.linear(px[:M, :K], pw[:N, :K], None, 0, None, sx, sw, F32)
+    assert bool(torch.isnan(got[M - 1]).all()) and torch.equal(got[:M - 1], clean[:M - 1])
+    one = x[5:6].expand(M, K)                                             # every row the same one in memory
+    sone = None if sx is None else sx[5:6].expand(M).contiguous()
+    got = ops.linear(one, w, None, 0, None, sone, sw, F32)
+    assert torch.equal(got, clean[5:6].expand(M, N))
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(1, 100, 256, F16), (20, 70, 4096, BF16), (130, 129, 64, E4M3), (300, 512, 128, BF16), (70, 60, 4096, F16),
+                                         (3000, 1028, 80, BF16), (3601, 3601, 1024, BF16), (3601, 3590, 2048, E4M3)])
 def test_linear_in_place_and_guards(M, N, K, dtype):
     """Through the C ABI: out may be the residual; what lies behind its rows and columns stays as it was."""
     import ctypes
@@ -550,6 +572,58 @@ def test_streams_and_graphs():
             for a, b in zip(head(ops, _lib, t), o):
                 assert torch.equal(a, b)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(3, 500, 700, BF16), (40, 200, 9000, F16), (300, 300, 200, E4M3), (3000, 1500, 256, F16),
+                                         (3600, 3600, 1024, BF16), (3600, 3600, 2048, E4M3)])
+def test_every_kernel_of_linear_in_a_graph_and_on_two_streams(M, N, K, dtype):
+    from compression_amd import ops
+    a, b = [operands(50 + i, M, N, K, dtype) for i in (0, 7)]
+    bias, res = rnd(51, N).to(DEV), rnd(52, M, N).to(BF16).to(DEV)
+
+    def run(t):
+        return ops.linear(t[0], t[1], bias, 6, res, t[2], t[3], BF16)
+    want = [run(a), run(b)]
+    graph = torch.cuda.CUDAGraph()
+    mine = [t.clone() if t is not None else None for t in a]
+    with torch.cuda.graph(graph):
+        out = run(mine)
+    for i in (0, 1, 1, 0):
+        for t, v in zip(mine, (a, b)[i]):
+            if t is not None:
+                t.copy_(v)
+        graph.replay()
+        assert torch.equal(out, want[i])
+        run(b)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    torch.cuda.synchronize()
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(run((a, b)[i % 2]))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 2])
+
+
+def test_balance_in_a_graph_by_itself():
+    """Captured forward and gradient, replayed on changed scores with other calls of the same operators between."""
+    from compression_amd import ops
+    for T, E, t in ((5000, 64, BF16), (77, 300, F32)):
+        for by_expert in (False, True):
+            base = [rnd(60 + i, T, E).to(t).to(DEV) for i in range(2)]
+            s = base[0].t().contiguous().t() if by_expert else base[0].clone()
+            other = rnd(63, 900, 33).to(DEV)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                loss, counts, n = ops.prior_balance(s, top_k=2)
+                grad = ops.prior_balance_grad(s, counts, n, top_k=2)
+            for i in (0, 1, 0):
+                s.copy_(base[i])
+                g.replay()
+                ops.prior_balance(other)
+                l, c, k = ops.prior_balance(s, top_k=2)
+                assert torch.equal(l, loss) and torch.equal(c, counts) and torch.equal(ops.prior_balance_grad(s, c, k, top_k=2), grad)
 
 
 def test_refusals():
