@@ -29,7 +29,6 @@ struct LinearArgs {
     char *out;
     int64_t rs, os;                   // in bytes
     int out_type, act;
-    int vec_out, vec_res;             // 16-byte accesses are possible
     int tiles_m, tiles_n;
     float *partial;                   // [splits][M][N] sums, where K is split
 };
@@ -81,10 +80,10 @@ __device__ __forceinline__ void take_row(const Vec (&rows)[ROWS][P], int m, Vec 
 // registers, so take is a switch over copies): unrolled it would be tens of KB of code.
 template <typename T, int MF, int V, typename Take>
 __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, int64_t n, Take take) {
-    constexpr int PER = 16 / sizeof(T), P = V / PER;
+    constexpr int PER = 16 / sizeof(T), P = V / PER, RUN = 8 / PER;         // values of a 16-byte piece, pieces of a lane and of a run
     typedef T vec_t __attribute__((ext_vector_type(PER)));
+    typedef vec_t vec_any __attribute__((aligned(sizeof(T))));              // (rows may begin at any element)
     auto col = [&](int i) { return n + (i & 7) + 32 * (i >> 3); };          // column of value i
-    const bool whole = col(V - 1) < a.N, vec_out = whole && a.vec_out, vec_res = a.res && whole && a.vec_res;
     float b[V], s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -98,20 +97,27 @@ __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, i
         const int64_t row = row0 + 16 * m < a.M ? row0 + 16 * m : a.M - 1;
         const T *r = (const T *)(a.res + row * a.rs);
 #pragma unroll
-        for (int i = 0; i < P; ++i) to[i] = *(const vec_t *)(r + col(i * PER));
+        for (int i = 0; i < P; ++i) {
+            if (col(i / RUN * 8 + 7) < a.N) {
+                to[i] = *(const vec_any *)(r + col(i * PER));
+            } else {                                          // a run that the row ends in, or before
+#pragma unroll
+                for (int q = 0; q < PER; ++q) to[i][q] = col(i * PER + q) < a.N ? r[col(i * PER + q)] : (T)0.0f;
+            }
+        }
     };
-    if (vec_res && KEPT == 1) fetch(0, ahead[0]);
+    if (a.res && KEPT == 1) fetch(0, ahead[0]);
 #pragma unroll 1
     for (int m = 0; m < MF; ++m) {
         const int64_t row = row0 + 16 * m;
-        if (vec_res && KEPT > 1 && m % KEPT == 0) {
+        if (a.res && KEPT > 1 && m % KEPT == 0) {
 #pragma unroll
             for (int i = 0; i < KEPT; ++i) fetch(m + i, ahead[i]);
         }
         float v[V];
         take(m, v);
         vec_t res[P];
-        if (vec_res) {
+        if (a.res) {
             take_row<KEPT, P>(ahead, m % KEPT, res);
             if (KEPT == 1 && m + 1 < MF) fetch(m + 1, ahead[0]);
         }
@@ -124,28 +130,23 @@ __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, i
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] += b[i];
         activate<V>(v, a.act);
-        if (vec_res) {
+        if (a.res) {
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] += (float)res[i / PER][i % PER];
-        } else if (a.res) {
-            const T *r = (const T *)(a.res + row * a.rs);
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (col(i) < a.N) v[i] += (float)r[col(i)];
         }
         T *o = (T *)(a.out + row * a.os);
-        if (vec_out) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                vec_t t;
+        for (int i = 0; i < P; ++i) {
+            vec_t t;
 #pragma unroll
-                for (int q = 0; q < PER; ++q) t[q] = (T)v[i * PER + q];
-                *(vec_t *)(o + col(i * PER)) = t;
+            for (int q = 0; q < PER; ++q) t[q] = (T)v[i * PER + q];
+            if (col(i / RUN * 8 + 7) < a.N) {
+                *(vec_any *)(o + col(i * PER)) = t;
+            } else {
+#pragma unroll
+                for (int q = 0; q < PER; ++q)
+                    if (col(i * PER + q) < a.N) o[col(i * PER + q)] = t[q];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (col(i) < a.N) o[col(i)] = (T)v[i];
         }
     }
 }
@@ -267,8 +268,8 @@ __device__ __forceinline__ u32x4 buffer_piece(rsrc_t r, unsigned offset) {
 
 // Workgroup (tile, split): BM x BN outputs over the split's k-tiles.  DEPTH k-tiles are on their way in registers while one
 // is worked on from LDS, so a tile of few rows, whose matrix instructions do not cover a memory access, is not bound by
-// it.  Operand rows may begin at any element, and are at least 16 bytes long.  The last k-tile, if the row ends inside
-// it, comes by itself behind the others: a piece past the row's end is loaded from its last 16 bytes and shifted.
+// it.  Operand rows may begin at any element.  The last k-tile, if the row ends inside it, comes by itself behind the others:
+// a piece past the row's end is loaded from its last 16 bytes and shifted.
 template <int TYPE, int BM, int BN, int WM, int WN, int DEPTH, int PER_SIMD>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_tile_kernel(LinearArgs a) {
     constexpr int NT = 64 * (BM / WM) * (BN / WN), TURN = DEPTH % 2 ? 2 * DEPTH : DEPTH;
@@ -380,12 +381,25 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_t
     }
 done:
     if (t1 > whole) {                                             // the tile in which the rows end
-        fetch(0, whole - t0);
-        const int over = whole * KT + p * 16 - (K - 16), sh = over < 0 ? 0 : over > 16 ? 16 : over;
+        if (K >= 16) {
+            fetch(0, whole - t0);
+            const int over = whole * KT + p * 16 - (K - 16), sh = over < 0 ? 0 : over > 16 ? 16 : over;
 #pragma unroll
-        for (int i = 0; i < XP; ++i) xr[0][i] = row_end(xr[0][i], sh);
+            for (int i = 0; i < XP; ++i) xr[0][i] = row_end(xr[0][i], sh);
 #pragma unroll
-        for (int i = 0; i < WP; ++i) wr[0][i] = row_end(wr[0][i], sh);
+            for (int i = 0; i < WP; ++i) wr[0][i] = row_end(wr[0][i], sh);
+        } else {                                                  // shorter than a piece: value by value
+#pragma unroll
+            for (int i = 0; i < XP; ++i) {
+                const int r = r0 + i * (NT / 8);
+                xr[0][i] = load_piece<Operand<TYPE>::BYTES>(a.x + (m0 + r) * a.xs, m0 + r < a.M ? K - p * 16 : 0);
+            }
+#pragma unroll
+            for (int i = 0; i < WP; ++i) {
+                const int r = r0 + i * (NT / 8);
+                wr[0][i] = load_piece<Operand<TYPE>::BYTES>(a.w + (n0 + r) * a.ws, n0 + r < a.N ? K - p * 16 : 0);
+            }
+        }
         stash(0, 0);
         lds_barrier();
         multiply(0, [] {});
@@ -397,7 +411,6 @@ done:
         sums.out = (char *)(a.partial + (int64_t)blockIdx.y * a.M * a.N);
         sums.os = a.N * 4;
         sums.out_type = MPC_TYPE_F32, sums.act = MPC_ACT_NONE;
-        sums.vec_out = a.N % 4 == 0;
         finish_rows<float, MF, V>(sums, m0 + wm + j, n0 + wn + g * 8, [&](int m, float (&v)[V]) { take_tile<MF, NF>(acc, m, v); });
         return;
     }
@@ -410,12 +423,12 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int spli
     if (i >= a.M * per_row) return;
     const int64_t m = i / per_row, n = i % per_row * 4, plane = a.M * a.N;
     const float *s = a.partial + m * a.N + n;
-    const bool whole = a.N % 4 == 0;                              // (then the rows are aligned as well)
+    typedef f32x4 f32x4_any __attribute__((aligned(4)));
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int z = 0; z < splits; ++z) {
-        if (whole) {
-            const f32x4 t = *(const f32x4 *)(s + z * plane);
+        if (n + 4 <= a.N) {
+            const f32x4 t = *(const f32x4_any *)(s + z * plane);
 #pragma unroll
             for (int c = 0; c < 4; ++c) v[c] += t[c];
         } else {
@@ -648,7 +661,7 @@ int launch_big(mpc_ctx *ctx, LinearArgs a, bool prepare = false) {
 // A workgroup takes 16 rows of w, its waves every WAVES-th k-tile of them, straight from memory into the registers of the
 // matrix instructions: no operand is used twice, so nothing goes through LDS but the waves' sums, which meet there in the
 // order of the waves.  UNITS k-tiles of a wave are in flight at once (64 KB and more per workgroup).  More rows than
-// MF tiles take more workgroups (only for the rows that no other kernel takes: see plan_for).
+// MF tiles take more workgroups (only for rows too far apart for the other kernels: see plan_for).
 template <int TYPE, int MF, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
     constexpr int UNITS = 4;
@@ -742,8 +755,8 @@ struct Plan {
 };
 
 Plan plan_for(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {     // the last three in bytes
-    // (rows shorter than a piece, or so far apart that a tile's do not fit a buffer: the kernel that addresses each by itself)
-    if (M <= 32 || K < 16 || BIG * xs + K > TILE_BYTES || BIG * ws + K > TILE_BYTES) return {PLAN_ROWS, 1};
+    // (rows so far apart that a tile's do not fit a buffer: the kernel that addresses each by itself)
+    if (M <= 32 || BIG * xs + K > TILE_BYTES || BIG * ws + K > TILE_BYTES) return {PLAN_ROWS, 1};
     const int64_t big = mpc_cdiv(M, BIG) * mpc_cdiv(N, BIG), middle = mpc_cdiv(M, 128) * mpc_cdiv(N, 128);
     // The large tile needs most CUs busy and some k-tiles to pay for its prologue and epilogue (128 x 128 tiles against it, bf16
     // with bias and gelu: 3584 x 4096 x 4096 137 us : 105; 2048 x 4096 x 4096 77 : 99; 4096 x 4096 x 1024 46 : 47; 8192 x 8192 x
@@ -836,8 +849,6 @@ extern "C" int mpc_linear_forward(mpc_ctx *ctx, const mpc_linear_desc *desc, con
     a.res = (const char *)residual, a.out = (char *)out;
     a.rs = d.residual_stride * ob, a.os = d.out_stride * ob;
     a.out_type = d.out_type, a.act = d.act;
-    a.vec_out = (uintptr_t)out % 16 == 0 && a.os % 16 == 0;
-    a.vec_res = (uintptr_t)residual % 16 == 0 && a.rs % 16 == 0;
     a.partial = (float *)workspace;
     if (d.in_type == MPC_TYPE_F16) return launch<MPC_TYPE_F16>(ctx, a);
     if (d.in_type == MPC_TYPE_BF16) return launch<MPC_TYPE_BF16>(ctx, a);
