@@ -200,7 +200,9 @@ class Context:
             raise MpcError(f"libmpc error {rc}: {msg.decode() if msg else ''}")
 
     def call(self, name: str, *args):
-        self.check(getattr(self.lib, name)(self.handle, *args))
+        rc = getattr(self.lib, name)(self.handle, *args)
+        if rc != 0:
+            self.check(rc)
 
     def close(self):
         if getattr(self, "handle", None):

@@ -43,10 +43,12 @@ __device__ __forceinline__ void activate(float (&v)[V], int act) {
     } else if (act == MPC_ACT_GELU) {
         // gelu(v) = max(v, 0) - |v| / 2 erfc(|v| / sqrt 2), with formula 7.1.26 of Abramowitz and Stegun (1964) for erfc, off by
         // at most 1.5e-7: erfc(u) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-u^2), t = 1 / (1 + p u).
-        // 13 instructions a value, where the library's erfc takes several times that.
+        // 14 instructions a value, where the library's erfc takes several times that.  |v| ends at 1e30 for v > 0 only, which
+        // makes gelu(inf) = inf; at -inf the formula's -inf * 0 is NaN, here as in silu.
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float m = fabsf(v[i]), t = __builtin_amdgcn_rcpf(fmaf(m, 0.3275911f * 0.70710678f, 1.0f));
+            const float m = fabsf(__builtin_fminf(v[i], 1e30f));
+            const float t = __builtin_amdgcn_rcpf(fmaf(m, 0.3275911f * 0.70710678f, 1.0f));
             float q = fmaf(t, -0.5f * 1.061405429f, 0.5f * 1.453152027f);                  // -erfc / (2 t exp)
             q = fmaf(t, q, -0.5f * 1.421413741f);
             q = fmaf(t, q, 0.5f * 0.284496736f);
@@ -802,11 +804,13 @@ int prepare(mpc_ctx *ctx) {
 
 bool linear_desc_ok(const mpc_linear_desc &d) {
     const bool in16 = d.in_type == MPC_TYPE_F16 || d.in_type == MPC_TYPE_BF16;
+    const int64_t far = 1ll << 40;             // elements: 256 rows of them are far from 63 bits of bytes
     return (in16 || d.in_type == MPC_TYPE_E4M3) &&
            (d.out_type == MPC_TYPE_F32 || d.out_type == MPC_TYPE_F16 || d.out_type == MPC_TYPE_BF16) &&
            (d.act == MPC_ACT_NONE || d.act == MPC_ACT_RELU || d.act == MPC_ACT_GELU || d.act == MPC_ACT_SILU) && d.M >= 0 &&
-           d.M < (1ll << 31) && d.N > 0 && d.N < (1ll << 31) && d.K > 0 && d.K < (1ll << 31) && d.x_stride >= 0 && d.w_stride >= 0 &&
-           d.residual_stride >= 0 && d.out_stride >= d.N;
+           d.M < (1ll << 31) && d.N > 0 && d.N < (1ll << 31) && d.K > 0 && d.K < (1ll << 31) && d.x_stride >= 0 && d.x_stride < far &&
+           d.w_stride >= 0 && d.w_stride < far && d.residual_stride >= 0 && d.residual_stride < far && d.out_stride >= d.N &&
+           d.out_stride < far;
 }
 
 }  // namespace

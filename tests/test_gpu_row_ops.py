@@ -248,6 +248,26 @@ def test_linear_strides_and_alignment(dtype, M):
     assert empty.shape == (0, N) and empty.dtype == F16
 
 
+@pytest.mark.parametrize("act", [0, 3, 5, 6])
+@pytest.mark.parametrize("M,N", [(4, 24), (24, 70), (100, 60), (2000, 2000), (4200, 3001)])
+def test_linear_infinite_and_largest_sums(act, M, N):
+    """Sums at the ends of fp32's range, through every kernel: the activations' own values there (gelu and silu of -inf are
+    NaN: -inf * 0)."""
+    from compression_amd import ops
+    K = 1032
+    ends = torch.tensor([math.inf, -math.inf, 3e38, -3e38, 1e30, -1e30, 1e4, -1e4, 100.0, -100.0, 0.0, -0.0, math.nan]).to(BF16).to(DEV)
+    x, w = torch.zeros(M, K, dtype=BF16, device=DEV), torch.zeros(N, K, dtype=BF16, device=DEV)
+    x[:, 5] = ends.repeat(M // len(ends) + 1)[:M]
+    w[:, 5] = 1.0
+    got = ops.linear(x, w, act=act, out_dtype=F32)
+    v = x[:, 5].double()
+    want = act64(v, act) if act != 6 else v / (1 + torch.exp(-v))
+    want = torch.where(want.abs() < 1e-30, 0.0, want).float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)[:, None].expand(M, N))
+    fin = ~torch.isnan(want)
+    assert torch.equal(torch.where(got[fin].abs() < 1e-30, 0.0, got[fin]), want[fin, None].expand(-1, N))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("M,K", [(1, 100), (6, 1111), (50, 260), (300, 72)])
 def test_linear_special_values_stay_where_they_are(dtype, M, K):

@@ -53,6 +53,14 @@ def test_linear_workspace_of_a_bad_description_is_zero():
     assert lib.mpc_prior_balance_workspace_bytes(0, 64) > 0
 
 
+def test_linear_refuses_strides_that_no_memory_has():
+    lib = _lib.load()
+    sizes = _lib.MPC_TYPE_BF16, _lib.MPC_TYPE_F32, 0, 64, 64, 1 << 16        # (a product whose K is split)
+    assert lib.mpc_linear_workspace_bytes(ctypes.byref(_lib.LinearDesc(*sizes, 1 << 16, 1 << 16, 0, 64))) > 0
+    for bad in ((1 << 61, 1 << 16, 0, 64), (1 << 16, 1 << 40, 0, 64), (1 << 16, 1 << 16, 1 << 62, 64), (1 << 16, 1 << 16, 0, 1 << 50)):
+        assert lib.mpc_linear_workspace_bytes(ctypes.byref(_lib.LinearDesc(*sizes, *bad))) == 0
+
+
 def test_entry_points_refuse_a_null_context():
     lib = _lib.load()
     d = _lib.LinearDesc(_lib.MPC_TYPE_F16, _lib.MPC_TYPE_F16, 0, 4, 4, 4, 4, 4, 0, 4)
