@@ -247,13 +247,18 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int &tm
     tn = in / rows;
 }
 
-// 16 bytes that begin `sh` bytes before the piece wanted (the row ends inside it, or before it): the piece, zeros behind the row
+// 16 bytes that begin `sh` bytes before the piece wanted (0 <= sh <= 16: the row ends inside it, or before it): the piece, zeros
+// behind the row
 __device__ __forceinline__ u32x4 row_end(u32x4 v, int sh) {
     typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
     u64x2 t = __builtin_bit_cast(u64x2, v);
-    if (sh >= 16) t[0] = t[1] = 0;
-    else if (sh >= 8) t[0] = t[1] >> (8 * sh - 64), t[1] = 0;
-    else if (sh > 0) t[0] = t[0] >> (8 * sh) | t[1] << (64 - 8 * sh), t[1] >>= 8 * sh;
+    t[0] = sh & 8 ? t[1] : t[0];
+    t[1] = sh & 8 ? 0 : t[1];
+    const int bits = 8 * (sh & 7);
+    t[0] = t[0] >> bits | t[1] << 1 << (63 - bits);
+    t[1] >>= bits;
+    t[0] = sh & 16 ? 0 : t[0];
+    t[1] = sh & 16 ? 0 : t[1];
     return __builtin_bit_cast(u32x4, t);
 }
 
@@ -270,8 +275,8 @@ __device__ __forceinline__ u32x4 buffer_piece(rsrc_t r, unsigned offset) {
 
 // Workgroup (tile, split): BM x BN outputs over the split's k-tiles.  DEPTH k-tiles are on their way in registers while one
 // is worked on from LDS, so a tile of few rows, whose matrix instructions do not cover a memory access, is not bound by
-// it.  Operand rows may begin at any element.  The last k-tile, if the row ends inside it, comes by itself behind the others:
-// a piece past the row's end is loaded from its last 16 bytes and shifted.
+// it.  Operand rows may begin at any element.  In the last k-tile, if the row ends inside it, a piece past the row's end is
+// loaded from its last 16 bytes and shifted.
 template <int TYPE, int BM, int BN, int WM, int WN, int DEPTH, int PER_SIMD>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_tile_kernel(LinearArgs a) {
     constexpr int NT = 64 * (BM / WM) * (BN / WN), TURN = DEPTH % 2 ? 2 * DEPTH : DEPTH;
@@ -286,10 +291,11 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_t
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
     const int rows_x = (int)(a.M - m0 < BM ? a.M - m0 : BM), rows_w = (int)(a.N - n0 < BN ? a.N - n0 : BN);
     const rsrc_t xb = tile_buffer(a.x + m0 * a.xs, rows_x, a.xs, a.K), wb = tile_buffer(a.w + n0 * a.ws, rows_w, a.ws, a.K);
-    // this split's k-tiles: T whole ones, and in the last split the one in which the rows end
+    // this split's k-tiles: T, the last split's last one being the one in which the rows end (if they end inside one)
     const int K = (int)a.K, whole = K / KT, all = (K + KT - 1) / KT;
     const int t0 = (int)((int64_t)all * blockIdx.y / gridDim.y), t1 = (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y);
-    const int T = (t1 < whole ? t1 : whole) - t0;
+    const int T = K >= 16 ? t1 - t0 : 0;
+    const bool ends = t1 > whole;
 
     // Piece p of row r lies at slot p ^ key(r): the 16 rows that one instruction reads at the same p then spread over the banks.
     auto xkey = [](int r) { return r & 7; };
@@ -303,6 +309,13 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_t
         for (int i = 0; i < XP; ++i) xr[slot][i] = buffer_piece(xb, xo + off + i * xstep);
 #pragma unroll
         for (int i = 0; i < WP; ++i) wr[slot][i] = buffer_piece(wb, wo + off + i * wstep);
+    };
+    const int over = whole * KT + p * 16 - (K - 16), sh = over < 0 ? 0 : over > 16 ? 16 : over;
+    auto finish = [&](int slot) {                                 // pieces of the tile in which the rows end
+#pragma unroll
+        for (int i = 0; i < XP; ++i) xr[slot][i] = row_end(xr[slot][i], sh);
+#pragma unroll
+        for (int i = 0; i < WP; ++i) wr[slot][i] = row_end(wr[slot][i], sh);
     };
     auto stash = [&](int slot, int buf) {
         u32x4 *x = lds + buf * (BM + BN) * 8, *w = x + BM * 8;
@@ -360,33 +373,37 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_t
     // Tile t from LDS buffer t & 1; tile t + 1 waits in slot (t + 1) % DEPTH.
     auto step = [&](int buf, int slot, int t) {
         multiply(buf, [&] {
+            if (DEPTH > 1 && ends && t + 2 == T) finish(slot);
             stash(slot, buf ^ 1);                                 // (last read before the previous barrier)
             fetch(slot, t + 1 + DEPTH);
         });
         lds_barrier();
     };
+    if (T > 0) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) fetch(d, d);
+        if (ends && T == 1) finish(0);
+        stash(0, 0);
+    }
     if constexpr (DEPTH == 1) {                                   // the only tile on its way is the one waited for
         if (T > 0) {
-            fetch(0, 0);
-            stash(0, 0);
             if (T > 1) fetch(0, 1);
             lds_barrier();
             int t = 0;
             for (; t + 2 < T; ++t) step(t & 1, 0, t);
             if (t + 1 < T) {
-                multiply(t & 1, [&] { stash(0, ~t & 1); });
+                multiply(t & 1, [&] {
+                    if (ends) finish(0);
+                    stash(0, ~t & 1);
+                });
                 lds_barrier();
                 ++t;
             }
             multiply(t & 1, [] {});
-            if (t1 > whole) lds_barrier();
         }
     } else if (T > 0) {
         // Tiles past the last are fetched and stored like the others, and never read: a fetch under a condition would make the
         // compiler wait for every load in flight, since it could not count on the younger ones.
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) fetch(d, d);
-        stash(0, 0);
         fetch(0, DEPTH);
         lds_barrier();
         for (int t = 0;; t += TURN) {
@@ -398,25 +415,16 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), PER_SIMD) void linear_t
         }
     }
 done:
-    if (t1 > whole) {                                             // the tile in which the rows end
-        if (K >= 16) {
-            fetch(0, whole - t0);
-            const int over = whole * KT + p * 16 - (K - 16), sh = over < 0 ? 0 : over > 16 ? 16 : over;
+    if (K < 16) {                                                 // rows shorter than a piece: value by value (in one split)
 #pragma unroll
-            for (int i = 0; i < XP; ++i) xr[0][i] = row_end(xr[0][i], sh);
+        for (int i = 0; i < XP; ++i) {
+            const int r = r0 + i * (NT / 8);
+            xr[0][i] = load_piece<Operand<TYPE>::BYTES>(a.x + (m0 + r) * a.xs, m0 + r < a.M ? K - p * 16 : 0);
+        }
 #pragma unroll
-            for (int i = 0; i < WP; ++i) wr[0][i] = row_end(wr[0][i], sh);
-        } else {                                                  // shorter than a piece: value by value
-#pragma unroll
-            for (int i = 0; i < XP; ++i) {
-                const int r = r0 + i * (NT / 8);
-                xr[0][i] = load_piece<Operand<TYPE>::BYTES>(a.x + (m0 + r) * a.xs, m0 + r < a.M ? K - p * 16 : 0);
-            }
-#pragma unroll
-            for (int i = 0; i < WP; ++i) {
-                const int r = r0 + i * (NT / 8);
-                wr[0][i] = load_piece<Operand<TYPE>::BYTES>(a.w + (n0 + r) * a.ws, n0 + r < a.N ? K - p * 16 : 0);
-            }
+        for (int i = 0; i < WP; ++i) {
+            const int r = r0 + i * (NT / 8);
+            wr[0][i] = load_piece<Operand<TYPE>::BYTES>(a.w + (n0 + r) * a.ws, n0 + r < a.N ? K - p * 16 : 0);
         }
         stash(0, 0);
         lds_barrier();
