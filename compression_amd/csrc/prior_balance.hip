@@ -7,6 +7,9 @@
 // wave keeps the sums of p of its rows in registers and counts choices in LDS; the blocks' sums meet in a second kernel,
 // in a fixed order and in double.  Scores whose experts are not consecutive (the competition writes its totals prior by
 // prior) go through an LDS tile, read and, for the gradient, written along the rows.
+//
+// 1M x 64 bf16, top 2, with a mask: forward 46 to 56 us, bound by its vector instructions (an exponential and two rounds of
+// the choice per score); gradient 48 to 51 us, 5.2 TB/s.  1536 x 64 fp32, expert by expert: 5.7 + 5.8 (join) + 5.3 us, latency.
 #include "row_ops.h"
 
 #include <type_traits>
