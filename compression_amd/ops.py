@@ -319,6 +319,11 @@ def _addr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _like(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A dense tensor of x's shape (empty_like takes 0.6 us less than a shape, but keeps the strides of a view)."""
+    return torch.empty_like(x, dtype=dtype) if x.is_contiguous() else x.new_empty(x.shape, dtype=dtype)
+
+
 # The wrappers below look a little bare: a call of a few rows takes the GPU 5-8 microseconds, and Python about as long.
 def _vector(t: torch.Tensor, n: int, name: str):
     if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
@@ -348,11 +353,12 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
         if residual.shape != x.shape or residual.dtype != dtype:
             raise MpcError(f"rms_norm: residual {residual.dtype} {tuple(residual.shape)} does not match x {dtype} {tuple(x.shape)}")
         _, rs = _rows(residual, "residual")
-        h = x.new_empty(x.shape)
+        h = _like(x, dtype)
     if quantize:
-        y, scale = x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32)
+        y = _like(x, torch.float8_e4m3fn)
+        scale = x.new_empty(rows, dtype=torch.float32) if x.dim() == 2 else x.new_empty(x.shape[:-1], dtype=torch.float32)
     else:
-        y, scale = x.new_empty(x.shape), None
+        y, scale = _like(x, dtype), None
     if rows:
         args = (x.data_ptr(), xs, _addr(residual), rs, _addr(weight), rows, C, eps, t, _addr(h), y.data_ptr(),
                 _lib.MPC_TYPE_E4M3 if quantize else t, _addr(scale))
@@ -406,7 +412,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         if residual.shape != shape or residual.dtype != odt:
             raise MpcError(f"linear: residual {residual.dtype} {tuple(residual.shape)} does not match the output {odt} {tuple(shape)}")
         _, rs = _rows(residual, "residual")
-    out = x.new_empty(shape, dtype=odt)
+    out = x.new_empty(*shape, dtype=odt)
     if M == 0:
         return out
     ctx = _lib.context_at(index)
