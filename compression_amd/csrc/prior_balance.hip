@@ -9,7 +9,7 @@
 // prior) go through an LDS tile, read and, for the gradient, written along the rows.
 //
 // 1M x 64 bf16, top 2, with a mask: forward 46 to 56 us, bound by its vector instructions (an exponential and two rounds of
-// the choice per score); gradient 48 to 51 us, 5.2 TB/s.  1536 x 64 fp32, expert by expert: 5.7 + 5.8 (join) + 5.3 us, latency.
+// the choice per score); gradient 48 to 51 us, 5.2 TB/s.  1536 x 64 fp32, expert by expert: 10 us with its join + 5.3, latency.
 #include "row_ops.h"
 
 #include <type_traits>
@@ -20,6 +20,8 @@ constexpr int PB_MAX_EXPERTS = 1024;
 constexpr int PB_MAX_THREADS = 512;
 constexpr int PB_WIDE_THREADS = 1024;   // forward kernel of consecutive experts (1M x 64 bf16, top 2: 56 us against 61 with 512)
 constexpr int PB_MAX_BLOCKS = 512;
+constexpr int PB_JOIN = 32;             // fewest experts of a workgroup of the join kernel
+constexpr int PB_HEAD = 2 * (1 + PB_MAX_EXPERTS / PB_JOIN);      // words in front of the blocks' sums: a ticket, a double per workgroup of the join
 
 struct Row {
     const void *scores;
@@ -203,7 +205,7 @@ __device__ __forceinline__ void stage(const Row &a, int64_t first, float *tile) 
     }
 }
 
-// words of a block in the workspace: sum of p (float) [experts], choices (int) [experts], rows (int)
+// words of a block in the workspace, behind the head: sum of p (float) [experts], choices (int) [experts], rows (int)
 template <typename T, int EPL, int LOG2, bool STAGED>
 __global__ __launch_bounds__(STAGED ? PB_MAX_THREADS : PB_WIDE_THREADS) void prior_balance_kernel(Row a, float *__restrict__ ws) {
     if constexpr (LOG2 >= 0) a.group = 1 << LOG2, a.group_log2 = LOG2;
@@ -213,6 +215,7 @@ __global__ __launch_bounds__(STAGED ? PB_MAX_THREADS : PB_WIDE_THREADS) void pri
     float *tile = lds + a.experts;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
     const int e0 = (lane & (a.group - 1)) * EPL, per_wave = 64 >> a.group_log2, per_block = per_wave * waves;
+    if (blockIdx.x == 0 && tid == 0) *(int *)ws = 0;          // (the join's ticket)
     for (int e = tid; e < a.experts; e += blockDim.x) hist[e] = 0;
     __syncthreads();
     float acc[EPL];
@@ -284,7 +287,7 @@ __global__ __launch_bounds__(STAGED ? PB_MAX_THREADS : PB_WIDE_THREADS) void pri
     }
     if (lane == 0) rsum[wave] = n;
     __syncthreads();
-    float *out = ws + (int64_t)blockIdx.x * (2 * a.experts + 1);
+    float *out = ws + PB_HEAD + (int64_t)blockIdx.x * (2 * a.experts + 1);
     for (int e = tid; e < a.experts; e += blockDim.x) {
         float s = 0.0f;
         for (int w = 0; w < waves; ++w) s += tile[w * width + e];
@@ -298,50 +301,71 @@ __global__ __launch_bounds__(STAGED ? PB_MAX_THREADS : PB_WIDE_THREADS) void pri
     }
 }
 
-// 1024 threads: `slices` of them add up the blocks of one expert
-__global__ __launch_bounds__(1024) void prior_balance_join_kernel(const float *__restrict__ ws, int blocks, int experts, int slices, int top_k,
-                                                                  float *__restrict__ loss, int32_t *__restrict__ counts,
-                                                                  int32_t *__restrict__ n_rows) {
-    __shared__ double psum[1024];
-    __shared__ int csum[1024];
-    __shared__ int nsum[16];
-    const int tid = threadIdx.x, words = 2 * experts + 1;
+// A workgroup adds up the blocks' sums of J experts, 1024 / J threads an expert.  The workgroup that finishes last (the ticket
+// says so) adds up their parts of the loss, in their order whichever it is.  Up to 64 experts take one workgroup, without a
+// ticket, more take 32 each (forward and join, one workgroup for all experts : this: 1000 x 700 47 us : 13, 10000 x 256 25 : 13;
+// one workgroup of 64 against two of 32: 1000 x 64 7.5 : 8.7; 32 against 64 at 10000 x 256: 12.6 : 14.2).
+template <int J>
+__global__ __launch_bounds__(1024) void prior_balance_join_kernel(float *__restrict__ ws, int blocks, int experts, int top_k,
+                                                                          float *__restrict__ loss, int32_t *__restrict__ counts,
+                                                                          int32_t *__restrict__ n_rows) {
+    constexpr int WAVES = 16;
+    __shared__ double psum[WAVES][J];
+    __shared__ int csum[WAVES][J], nsum[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, words = 2 * experts + 1;
+    const float *sums = ws + PB_HEAD;
     int n = 0;
-    for (int b = tid; b < blocks; b += 1024) n += ((const int *)ws)[(int64_t)b * words + 2 * experts];
-    for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-    if ((tid & 63) == 0) nsum[tid >> 6] = n;
-    const int slice = tid / experts, e = tid - slice * experts;
+    for (int b = tid; b < blocks; b += 1024) n += ((const int *)sums)[(int64_t)b * words + 2 * experts];
+    const int at = tid % J, e = blockIdx.x * J + at;
     double p = 0.0;
     int c = 0;
-    if (slice < slices) {
-#pragma unroll 8
-        for (int b = slice; b < blocks; b += slices) {
-            p += (double)ws[(int64_t)b * words + e];
-            c += ((const int *)ws)[(int64_t)b * words + experts + e];
+    constexpr int U = 8, STEP = 1024 / J;               // loads of eight blocks at once
+    for (int b0 = tid / J; b0 < blocks; b0 += U * STEP) {
+        float x[U];
+        int y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t from = (int64_t)(b0 + u * STEP < blocks ? b0 + u * STEP : b0) * words + (e < experts ? e : 0);
+            x[u] = sums[from], y[u] = ((const int *)sums)[from + experts];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b0 + u * STEP < blocks) p += (double)x[u], c += y[u];
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+        n += __shfl_xor(n, off, 64);
+        if (off >= J) p += __shfl_xor(p, off, 64), c += __shfl_xor(c, off, 64);
+    }
+    if (lane < J) psum[wave][lane] = p, csum[wave][lane] = c;
+    if (lane == 0) nsum[wave] = n;
+    __syncthreads();
+    if (wave > 0) return;
+    p = 0.0, c = 0, n = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) p += psum[w][at], c += csum[w][at], n += nsum[w];
+    if (lane < J && e < experts) counts[e] = c;
+    double term = lane < J && e < experts && n > 0 ? (double)c / ((double)top_k * n) * (p / n) : 0.0;
+    auto total = [&] {
+        for (int off = 32; off > 0; off >>= 1) term += __shfl_xor(term, off, 64);
+    };
+    total();
+    int last = 1;
+    if (gridDim.x > 1) {
+        uint64_t *terms = (uint64_t *)ws + 1;
+        if (lane == 0) {
+            __hip_atomic_store(terms + blockIdx.x, __builtin_bit_cast(uint64_t, term), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = __hip_atomic_fetch_add((int *)ws, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+        }
+        last = __shfl(last, 0, 64);
+        if (last) {
+            __atomic_thread_fence(__ATOMIC_ACQUIRE);
+            term = lane < (int)gridDim.x ? __builtin_bit_cast(double, __hip_atomic_load(terms + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) : 0.0;
+            total();
         }
     }
-    psum[tid] = p;
-    csum[tid] = c;
-    __syncthreads();
-    n = 0;
-    for (int w = 0; w < 16; ++w) n += nsum[w];
-    double term = 0.0;
-    if (tid < experts) {
-        for (int s = 1; s < slices; ++s) p += psum[s * experts + tid], c += csum[s * experts + tid];
-        counts[tid] = c;
-        if (n > 0) term = (double)c / ((double)top_k * n) * (p / n);
-    }
-    __syncthreads();
-    for (int off = 32; off > 0; off >>= 1) term += __shfl_xor(term, off, 64);
-    if ((tid & 63) == 0) psum[tid >> 6] = term;
-    __syncthreads();
-    if (tid == 0) {
-        double s = 0.0;
-        for (int w = 0; w < 16; ++w) s += psum[w];
-        *loss = (float)(experts * s);
-        *n_rows = n;
-    }
+    if (last && lane == 0) *loss = (float)(experts * term), *n_rows = n;
 }
+static_assert(PB_MAX_EXPERTS / PB_JOIN <= 64, "a wave adds up the workgroups' parts");
 
 template <typename T, int EPL, int LOG2, bool STAGED>
 __global__ __launch_bounds__(PB_MAX_THREADS) void prior_balance_grad_kernel(Row a, const int32_t *__restrict__ counts,
@@ -463,8 +487,10 @@ struct Shape {
     size_t tile_bytes;
 };
 
-// Lanes per row, rows per tile, threads per block.  Few rows: small blocks, so that more CUs take part.
-Shape shape(Row &a, bool staged, int most) {
+// Lanes per row, rows per tile, threads per block.  Few rows: small blocks (`least` threads), so that more CUs take part; not as
+// small in the forward kernel, whose blocks are joined afterwards (10000 x 256, 128 threads : 512: 16.5 us : 14.5, the gradient
+// 9.0 : 11.3).
+Shape shape(Row &a, bool staged, int least, int most) {
     Shape s{};
     s.epl = a.experts > 8 * 64 ? 16 : 8;
     a.group = 1, a.group_log2 = 0;
@@ -482,7 +508,7 @@ Shape shape(Row &a, bool staged, int most) {
         s.tile_bytes = (size_t)r * (a.experts + 1) * sizeof(float);
         per_block = r;
     } else {
-        s.threads = few ? 128 : most;
+        s.threads = few ? least : most;
         per_block = s.threads / a.group;
     }
     s.passes = a.rows > 0 ? mpc_cdiv(a.rows, per_block) : 1;
@@ -506,7 +532,7 @@ void by_group(int log2, F f) {
 template <typename T>
 int forward(mpc_ctx *ctx, Row a, float *ws, float *loss, int32_t *counts, int32_t *n_rows) {
     const bool staged = a.expert_stride != 1 && a.experts > 1;
-    const Shape s = shape(a, staged, PB_WIDE_THREADS);
+    const Shape s = shape(a, staged, 512, PB_WIDE_THREADS);
     const int blocks = (int)(s.passes > PB_MAX_BLOCKS ? PB_MAX_BLOCKS : s.passes);
     size_t sums = (size_t)(s.threads / 64) * a.group * s.epl * sizeof(float);
     if (sums < s.tile_bytes) sums = s.tile_bytes;
@@ -517,7 +543,10 @@ int forward(mpc_ctx *ctx, Row a, float *ws, float *loss, int32_t *counts, int32_
     else if (s.epl == 16) run(prior_balance_kernel<T, 16, 6, false>);
     else by_group(a.group_log2, [&](auto log2) { run(prior_balance_kernel<T, 8, decltype(log2)::value, false>); });
     MPC_CHECK_LAUNCH(ctx, "prior_balance");
-    prior_balance_join_kernel<<<dim3(1), dim3(1024), 0, ctx->stream>>>(ws, blocks, a.experts, 1024 / a.experts, a.top_k, loss, counts, n_rows);
+    const dim3 all(1024);
+    if (a.experts <= 64) prior_balance_join_kernel<64><<<dim3(1), all, 0, ctx->stream>>>(ws, blocks, a.experts, a.top_k, loss, counts, n_rows);
+    else prior_balance_join_kernel<PB_JOIN><<<dim3((unsigned)mpc_cdiv(a.experts, PB_JOIN)), all, 0, ctx->stream>>>(ws, blocks, a.experts, a.top_k, loss,
+                                                                                                                  counts, n_rows);
     MPC_CHECK_LAUNCH(ctx, "prior_balance_join");
     return MPC_OK;
 }
@@ -525,7 +554,7 @@ int forward(mpc_ctx *ctx, Row a, float *ws, float *loss, int32_t *counts, int32_
 template <typename T>
 int backward(mpc_ctx *ctx, Row a, const int32_t *counts, const int32_t *n_rows, const float *grad_out, void *grad, int64_t grs, int64_t ges) {
     const bool staged = a.expert_stride != 1 && a.experts > 1;
-    const Shape s = shape(a, staged, PB_MAX_THREADS);
+    const Shape s = shape(a, staged, 128, PB_MAX_THREADS);
     const dim3 grid((unsigned)(s.passes > 1024 ? 1024 : s.passes)), block(s.threads);
     T *o = (T *)grad;
     auto run = [&](auto kernel) { kernel<<<grid, block, staged ? s.tile_bytes : 0, ctx->stream>>>(a, counts, n_rows, grad_out, o, grs, ges); };
@@ -553,7 +582,7 @@ extern "C" size_t mpc_prior_balance_workspace_bytes(int64_t rows, int experts) {
     if (rows < 0 || experts <= 0 || experts > PB_MAX_EXPERTS) return 0;
     // as many blocks as either layout's kernel may take for these rows
     const int64_t blocks = mpc_cdiv(rows, 2) + 1;
-    return (size_t)(blocks > PB_MAX_BLOCKS ? PB_MAX_BLOCKS : blocks) * (2 * experts + 1) * sizeof(float);
+    return (PB_HEAD + (size_t)(blocks > PB_MAX_BLOCKS ? PB_MAX_BLOCKS : blocks) * (2 * experts + 1)) * sizeof(float);
 }
 
 extern "C" int mpc_prior_balance(mpc_ctx *ctx, const void *scores, int type, int64_t rows, int experts, int64_t row_stride,
@@ -562,7 +591,7 @@ extern "C" int mpc_prior_balance(mpc_ctx *ctx, const void *scores, int type, int
     MPC_ENTER(ctx);
     const int bad = check(ctx, scores, type, rows, experts, row_stride, expert_stride, scale, top_k);
     if (bad) return bad;
-    MPC_REQUIRE(ctx, workspace && loss && counts && n_rows && ((uintptr_t)workspace & 3) == 0, "prior_balance: null or misaligned pointer");
+    MPC_REQUIRE(ctx, workspace && loss && counts && n_rows && ((uintptr_t)workspace & 7) == 0, "prior_balance: null or misaligned pointer");
     MPC_REQUIRE(ctx, workspace_bytes >= mpc_prior_balance_workspace_bytes(rows, experts), "prior_balance: workspace of %zu bytes", workspace_bytes);
     const Row a{scores, rows, row_stride, expert_stride, experts, scale, top_k, mask};
     if (type == MPC_TYPE_F32) return forward<float>(ctx, a, (float *)workspace, loss, counts, n_rows);

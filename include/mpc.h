@@ -384,7 +384,7 @@ int mpc_linear_forward(mpc_ctx *ctx, const mpc_linear_desc *desc, const void *x,
  * The gradient takes f as a constant:
  *   grad[row][j] = grad_out * scale * experts / R * p[j] (f[j] - sum_e f[e] p[e]),  0 in rows that do not count.
  * counts int32 [experts], n_rows int32 [1] (R), loss fp32 [1], all on the device; grad_out fp32 [1] on the device (NULL:
- * 1).  rows * top_k < 2^31, experts <= 1024, 1 <= top_k <= experts; rows may be 0.  The order of every sum is fixed: the
+ * 1).  workspace 8-byte aligned.  rows * top_k < 2^31, experts <= 1024, 1 <= top_k <= experts; rows may be 0.  The order of every sum is fixed: the
  * same call gives the same bits.  Replaces nothing of the reference: its remedy for idle priors is forcing them onto
  * locations (manynets_compressor.py:583-607). */
 size_t mpc_prior_balance_workspace_bytes(int64_t rows, int experts);
