@@ -722,7 +722,23 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
 #pragma unroll
                     for (int m = 0; m < MF; ++m) xv[i][m][c] = *(const u32x4_any *)(x[m] + k + c * 64);
                 }
-            } else {                                          // the row's end, or past it: zeros
+            } else if (k >= a.K) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    wv[i][c] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int m = 0; m < MF; ++m) xv[i][m][c] = u32x4{0, 0, 0, 0};
+                }
+            } else if (a.K >= 16) {                           // the row ends in this one
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int64_t at = k + c * 64, over = at + g * 16 - (a.K - 16), back = over > 0 ? over : 0;
+                    const int sh = (int)(back < 16 ? back : 16);
+                    wv[i][c] = row_end(*(const u32x4_any *)(w + at - back), sh);
+#pragma unroll
+                    for (int m = 0; m < MF; ++m) xv[i][m][c] = row_end(*(const u32x4_any *)(x[m] + at - back), sh);
+                }
+            } else {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int64_t left = a.K - k - c * 64 - g * 16;
