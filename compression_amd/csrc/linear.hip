@@ -21,6 +21,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x8 __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4_any __attribute__((aligned(1)));          // a 16-byte access at any address
+typedef u32x4 u32x4_word __attribute__((aligned(4)));         // at any word
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
@@ -267,6 +268,14 @@ __device__ __forceinline__ u32x4 row_end(u32x4 v, int sh) {
     t[0] = sh & 16 ? 0 : t[0];
     t[1] = sh & 16 ? 0 : t[1];
     return __builtin_bit_cast(u32x4, t);
+}
+
+// The 16 bytes at an address that is `s` (0 to 3) bytes behind a multiple of 4, from the 16 at the multiple and the word behind them.
+// Few rows, bound by memory: 3 x 8191 -> 8192 bf16 63 us with loads at such addresses, 34 with these.  (The tiles of the other
+// kernels do not gain: 8000 x 1089 -> 4000 103 us : 130.)
+__device__ __forceinline__ u32x4 from_words(u32x4 v, unsigned next, unsigned s) {
+    return u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], s), __builtin_amdgcn_alignbyte(v[2], v[1], s), __builtin_amdgcn_alignbyte(v[3], v[2], s),
+                 __builtin_amdgcn_alignbyte(next, v[3], s)};
 }
 
 // A tile's rows of an operand as a buffer that ends with the last row: a load for a row past it gives zeros or, where rows
@@ -694,10 +703,11 @@ int launch_big(mpc_ctx *ctx, LinearArgs a, bool prepare = false) {
 // A workgroup takes 16 rows of w, its waves every WAVES-th k-tile of them, straight from memory into the registers of the
 // matrix instructions: no operand is used twice, so nothing goes through LDS but the waves' sums, which meet there in the
 // order of the waves.  UNITS k-tiles of a wave are in flight at once (64 KB and more per workgroup).  More rows than
-// MF tiles take more workgroups (only for rows too far apart for the other kernels: see plan_for).
-template <int TYPE, int MF, int WAVES>
+// MF tiles take more workgroups (only for rows too far apart for the other kernels: see plan_for).  ODD: rows that begin between
+// words; a word that holds a byte of the row is all that is read besides it.
+template <int TYPE, int MF, int WAVES, bool ODD>
 __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
-    constexpr int UNITS = 4;
+    constexpr int UNITS = ODD && MF == 2 && WAVES == 16 ? 2 : 4, NEXT = ODD ? UNITS : 1;      // (four would not fit the registers there)
     __shared__ f32x4 part[WAVES * MF * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 15, g = lane >> 4;
@@ -705,12 +715,22 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
     const char *w = a.w + (n0 + j < a.N ? n0 + j : a.N - 1) * a.ws + g * 16, *x[MF];
 #pragma unroll
     for (int m = 0; m < MF; ++m) x[m] = a.x + (m0 + m * 16 + j < a.M ? m0 + m * 16 + j : a.M - 1) * a.xs + g * 16;
+    const unsigned wodd = (unsigned)((uintptr_t)w & 3);
+    unsigned xodd[MF];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) xodd[m] = (unsigned)((uintptr_t)x[m] & 3);
     f32x4 acc[MF];
 #pragma unroll
     for (int m = 0; m < MF; ++m) acc[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int units = (int)((a.K + KT - 1) / KT);
     for (int first = wave; first < units; first += WAVES * UNITS) {
         u32x4 wv[UNITS][2], xv[UNITS][MF][2];
+        unsigned wnext[NEXT][2], xnext[NEXT][MF][2];
+        // (the word behind the 16 bytes if it holds one of those wanted, else the last of the 16)
+        auto piece = [](const char *from, unsigned odd, u32x4 &v, unsigned &next) {
+            v = *(const u32x4_word *)(from - odd);
+            next = *(const unsigned *)(from - odd + (odd ? 16 : 12));
+        };
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
             const int u = first + i * WAVES;
@@ -718,9 +738,15 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
             if (k + KT <= a.K) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    wv[i][c] = *(const u32x4_any *)(w + k + c * 64);
+                    if constexpr (ODD) {
+                        piece(w + k + c * 64, wodd, wv[i][c], wnext[i][c]);
 #pragma unroll
-                    for (int m = 0; m < MF; ++m) xv[i][m][c] = *(const u32x4_any *)(x[m] + k + c * 64);
+                        for (int m = 0; m < MF; ++m) piece(x[m] + k + c * 64, xodd[m], xv[i][m][c], xnext[i][m][c]);
+                    } else {
+                        wv[i][c] = *(const u32x4_any *)(w + k + c * 64);
+#pragma unroll
+                        for (int m = 0; m < MF; ++m) xv[i][m][c] = *(const u32x4_any *)(x[m] + k + c * 64);
+                    }
                 }
             } else if (k >= a.K) {
 #pragma unroll
@@ -734,9 +760,17 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
                 for (int c = 0; c < 2; ++c) {
                     const int64_t at = k + c * 64, over = at + g * 16 - (a.K - 16), back = over > 0 ? over : 0;
                     const int sh = (int)(back < 16 ? back : 16);
-                    wv[i][c] = row_end(*(const u32x4_any *)(w + at - back), sh);
+                    auto last = [&](const char *from) {
+                        if constexpr (!ODD) return row_end(*(const u32x4_any *)from, sh);
+                        u32x4 v;
+                        unsigned next;
+                        const unsigned odd = (unsigned)((uintptr_t)from & 3);
+                        piece(from, odd, v, next);
+                        return row_end(from_words(v, next, odd), sh);
+                    };
+                    wv[i][c] = last(w + at - back);
 #pragma unroll
-                    for (int m = 0; m < MF; ++m) xv[i][m][c] = row_end(*(const u32x4_any *)(x[m] + at - back), sh);
+                    for (int m = 0; m < MF; ++m) xv[i][m][c] = last(x[m] + at - back);
                 }
             } else {
 #pragma unroll
@@ -749,7 +783,15 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < UNITS; ++i)
+        for (int i = 0; i < UNITS; ++i) {
+            if (ODD && (int64_t)(first + i * WAVES + 1) * KT <= a.K) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    wv[i][c] = from_words(wv[i][c], wnext[i % NEXT][c], wodd);
+#pragma unroll
+                    for (int m = 0; m < MF; ++m) xv[i][m][c] = from_words(xv[i][m][c], xnext[i % NEXT][m][c], xodd[m]);
+                }
+            }
 #pragma unroll
             for (int m = 0; m < MF; ++m) {
                 if constexpr (TYPE == MPC_TYPE_E4M3) {
@@ -759,6 +801,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
                     acc[m] = Operand<TYPE>::mma(wv[i][1], xv[i][m][1], acc[m]);
                 }
             }
+        }
     }
     // [wave][16 MF rows][16 columns]
 #pragma unroll
@@ -780,14 +823,17 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
     }
 }
 
-template <int TYPE, int MF>
+// rows that begin between words
+bool between_words(const LinearArgs &a) { return ((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.xs | (uintptr_t)a.ws) % 4 != 0; }
+
+template <int TYPE, int MF, bool ODD>
 int launch_rows(mpc_ctx *ctx, LinearArgs a) {
     const int64_t tiles_n = mpc_cdiv(a.N, 16), blocks = tiles_n * mpc_cdiv(a.M, 16 * MF);
     MPC_REQUIRE(ctx, blocks < (1ll << 31), "linear: too many tiles");
     a.tiles_n = (int)tiles_n;
     // up to a workgroup per CU: 16 waves, so that the CU's whole share of w is on its way; more: 8 waves, two workgroups a CU
-    if (blocks <= 256) linear_rows_kernel<TYPE, MF, 16><<<dim3((unsigned)blocks), dim3(1024), 0, ctx->stream>>>(a);
-    else linear_rows_kernel<TYPE, MF, 8><<<dim3((unsigned)blocks), dim3(512), 0, ctx->stream>>>(a);
+    if (blocks <= 256) linear_rows_kernel<TYPE, MF, 16, ODD><<<dim3((unsigned)blocks), dim3(1024), 0, ctx->stream>>>(a);
+    else linear_rows_kernel<TYPE, MF, 8, ODD><<<dim3((unsigned)blocks), dim3(512), 0, ctx->stream>>>(a);
     MPC_CHECK_LAUNCH(ctx, "linear_rows");
     return MPC_OK;
 }
@@ -835,7 +881,10 @@ int launch_middle(mpc_ctx *ctx, const LinearArgs &a, bool prepare = false) {
 template <int TYPE>
 int launch(mpc_ctx *ctx, const LinearArgs &a) {
     const Plan plan = plan_for(a.M, a.N, a.K, a.xs, a.ws);
-    if (plan.kind == PLAN_ROWS) return a.M <= 16 ? launch_rows<TYPE, 1>(ctx, a) : launch_rows<TYPE, 2>(ctx, a);
+    if (plan.kind == PLAN_ROWS) {
+        if (between_words(a)) return a.M <= 16 ? launch_rows<TYPE, 1, true>(ctx, a) : launch_rows<TYPE, 2, true>(ctx, a);
+        return a.M <= 16 ? launch_rows<TYPE, 1, false>(ctx, a) : launch_rows<TYPE, 2, false>(ctx, a);
+    }
     if (plan.kind == PLAN_BIG && big_possible(a)) return launch_big<TYPE>(ctx, a);
     if (plan.kind == PLAN_SMALL) return launch_small<TYPE>(ctx, a, plan.splits);
     return launch_middle<TYPE>(ctx, a);
