@@ -563,9 +563,10 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
     const unsigned xo = r0 * (unsigned)a.xs + p * 16, wo = r0 * (unsigned)a.ws + p * 16;
     const unsigned xstep = 32 * (unsigned)a.xs, wstep = 32 * (unsigned)a.ws;
     u32x4 xg[8], wg[8];
-    const int K = (int)a.K;
-    // (a piece past K, a multiple of 16 bytes here, gets an offset past the end: zeros)
-    auto k_offset = [&](int k) { return k + p * 16 < K ? (unsigned)k : 0x80000000u; };
+    // The last k-tile, which may end early, comes first, before the loop: it takes care of its end there.  The others follow,
+    // and tiles of zeros (from behind the buffer) behind them.
+    const int K = (int)a.K, last = (K - 1) / KT * KT, all = last + KT;
+    auto k_offset = [&](int k) { return k < all ? (unsigned)(k - KT) : 0x80000000u; };
     auto fetch_x = [&](int i, unsigned ko) { xg[i] = buffer_piece(xr, xo + ko + i * xstep); };
     auto fetch_w = [&](int i, unsigned ko) { wg[i] = buffer_piece(wr, wo + ko + i * wstep); };
     // LDS slots, as in the kernel above: piece p of row r at p ^ key(r); rows of w are read interleaved, so its
@@ -632,7 +633,7 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
         const unsigned ko = k_offset(k2), ko3 = k_offset(k2 + KT);
         if constexpr (TYPE == MPC_TYPE_E4M3) {
             asm volatile("" ::"v"(line));                     // (the line asked for a tile ago; older than pieces waited for below)
-            line = __builtin_amdgcn_raw_buffer_load_b32(lr, lo + (k2 + AHEAD * KT < K ? (unsigned)(k2 + AHEAD * KT) : 0x80000000u), 0, 0);
+            line = __builtin_amdgcn_raw_buffer_load_b32(lr, lo + k_offset(k2 + AHEAD * KT), 0, 0);
         }
         multiply(wa, x0, ha, Lo{}, [&](int i) {
             if (i < 4) read_w(wb, 2 * i, buf, WB), read_w(wb, 2 * i + 1, buf, WB);
@@ -654,9 +655,14 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
             if (i % 2 == 0) move(i / 2, buf, ko3);
         });
     };
-    const unsigned k0 = k_offset(0), k1 = k_offset(KT);
+    const int past = last + p * 16 - (K - 16), back = past > 0 ? past : 0;
+    const unsigned k0 = last - back, k1 = k_offset(KT);
 #pragma unroll
     for (int i = 0; i < 8; ++i) fetch_x(i, k0), fetch_w(i, k0);
+    if (K % KT != 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xg[i] = row_end(xg[i], back < 16 ? back : 16), wg[i] = row_end(wg[i], back < 16 ? back : 16);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) stash_x(i, 0), stash_w(i, 0);
 #pragma unroll
@@ -678,7 +684,7 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
         tile(0, k + 2 * KT, w0, w1, Lo{}, Hi{});
         tile(1, k + 3 * KT, w1, w0, Hi{}, Lo{});
         k += 2 * KT;
-    } while (k < K);
+    } while (k < all);
     // The compiler does not see that the last instructions above write accumulators: their results are complete behind this.
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
@@ -838,11 +844,6 @@ int launch_rows(mpc_ctx *ctx, LinearArgs a) {
     return MPC_OK;
 }
 
-// 16-byte pieces everywhere
-bool big_possible(const LinearArgs &a) {
-    return ((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.xs | (uintptr_t)a.ws | (uintptr_t)a.K) % 16 == 0;
-}
-
 // ---- which kernel ---------------------------------------------------------------------------------------------------------------
 enum { PLAN_ROWS, PLAN_SMALL, PLAN_MIDDLE, PLAN_BIG };
 struct Plan {
@@ -885,7 +886,7 @@ int launch(mpc_ctx *ctx, const LinearArgs &a) {
         if (between_words(a)) return a.M <= 16 ? launch_rows<TYPE, 1, true>(ctx, a) : launch_rows<TYPE, 2, true>(ctx, a);
         return a.M <= 16 ? launch_rows<TYPE, 1, false>(ctx, a) : launch_rows<TYPE, 2, false>(ctx, a);
     }
-    if (plan.kind == PLAN_BIG && big_possible(a)) return launch_big<TYPE>(ctx, a);
+    if (plan.kind == PLAN_BIG) return launch_big<TYPE>(ctx, a);
     if (plan.kind == PLAN_SMALL) return launch_small<TYPE>(ctx, a, plan.splits);
     return launch_middle<TYPE>(ctx, a);
 }

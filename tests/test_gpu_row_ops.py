@@ -225,6 +225,27 @@ def test_linear_large(dtype, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("K", [2048, 2049, 2055, 2063, 2064, 2175, 2176, 2177, 4225])
+def test_large_tiles_whose_rows_end_anywhere(dtype, K):
+    """256 x 256 tiles over rows of any length and at any address: small whole operands as above, NaN behind every row, in
+    front of it and behind the last one."""
+    from compression_amd import ops
+    M = N = 3590
+    g = torch.Generator().manual_seed(K)
+    nan = torch.full((M + 1, K + 5), float("nan"))
+    for lo in (0, 1, 5):
+        x, w = nan.clone(), nan.clone()
+        x[:M, lo:lo + K] = torch.randint(-4, 5, (M, K), generator=g).float()
+        w[:N, lo:lo + K] = torch.randint(-4, 5, (N, K), generator=g).float()
+        x, w = x.to(DEV), w.to(DEV)
+        xs, ws = x.to(dtype)[:M, lo:lo + K], w.to(dtype)[:N, lo:lo + K]
+        one = torch.ones(M, device=DEV) if dtype == E4M3 else None
+        got = ops.linear(xs, ws, x_scale=one, weight_scale=one, out_dtype=F32)
+        want = x[:M, lo:lo + K] @ w[:N, lo:lo + K].t().contiguous()           # (exact in fp32 as well)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("M", [1, 5, 40, 200])
 def test_linear_strides_and_alignment(dtype, M):
     """Slices of wider rows, rows that start at any element, broadcast rows, leading axes, and no copy of any of them."""
