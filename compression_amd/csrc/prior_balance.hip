@@ -53,15 +53,22 @@ __device__ __forceinline__ T group_reduce(T v, int group, Op op) {
     if (group > 2) v = op(v, dpp<0x4E>(v));
     if (group > 4) v = op(v, dpp<0x141>(v));
     if (group > 8) v = op(v, dpp<0x140>(v));
-    if (group > 16) v = op(v, __shfl_xor(v, 16, 64));
-    if (group > 32) v = op(v, __shfl_xor(v, 32, 64));
+    // rows of 16 lanes 0 0 2 2 and 1 1 3 3, then halves 0 0 and 1 1 (a swap reads what the instruction two before it wrote; the
+    // compiler's builtins take the two results for one)
+    if (group > 16) {
+        T w = v;
+        asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+        v = op(v, w);
+    }
+    if (group > 32) {
+        T w = v;
+        asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+        v = op(v, w);
+    }
     return v;
 }
 struct Max {
     __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
-};
-struct Min {
-    __device__ __forceinline__ int operator()(int a, int b) const { return a < b ? a : b; }
 };
 struct Add {
     __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
@@ -223,6 +230,7 @@ __global__ __launch_bounds__(STAGED ? PB_MAX_THREADS : PB_WIDE_THREADS) void pri
 #pragma unroll
     for (int j = 0; j < EPL; ++j) acc[j] = 0.0f;
 
+    const uint64_t before = (1ull << lane) - (1ull << (lane & ~(a.group - 1)));              // the lanes in front of this one in its group
     auto one = [&](bool keep, float (&v)[EPL]) {
         float e[EPL], top, inv;
         keep = softmax<LOG2, EPL>(a, keep, v, e, top, inv);
@@ -237,14 +245,15 @@ __global__ __launch_bounds__(STAGED ? PB_MAX_THREADS : PB_WIDE_THREADS) void pri
                 for (int j = 1; j < EPL; ++j) best = fmaxf(best, v[j]);
                 best = group_reduce<LOG2>(best, a.group, Max());
             }
-            int at_e = PB_MAX_EXPERTS;
+            int at = EPL;
 #pragma unroll
-            for (int j = EPL - 1; j >= 0; --j) at_e = v[j] == best ? e0 + j : at_e;
-            at_e = group_reduce<LOG2>(at_e, a.group, Min());
-            if (keep && best > -INFINITY && e0 == 0) atomicAdd(&hist[at_e], 1);
+            for (int j = EPL - 1; j >= 0; --j) at = v[j] == best ? j : at;
+            // the group's first lane that holds it chooses
+            at = __ballot(at < EPL) & before ? EPL : at;
+            if (keep && best > -INFINITY && at < EPL) atomicAdd(&hist[e0 + at], 1);
             if (k + 1 < a.top_k) {
 #pragma unroll
-                for (int j = 0; j < EPL; ++j) v[j] = e0 + j == at_e ? -INFINITY : v[j];
+                for (int j = 0; j < EPL; ++j) v[j] = j == at ? -INFINITY : v[j];
             }
         }
     };
