@@ -858,7 +858,9 @@ Plan plan_for(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {     // 
     // with bias and gelu: 3584 x 4096 x 4096 137 us : 105; 2048 x 4096 x 4096 77 : 99; 4096 x 4096 x 1024 46 : 47; 8192 x 8192 x
     // 512 114 : 119).  64 x 64 tiles take over where 128 x 128 ones are fewer than the CUs (768 x 4096 x 4096 44 : 39; 512 x 4096 x
     // 4096 32 : 39).
-    if (big >= 192 && K >= 2048) return {PLAN_BIG, 1};
+    // A turn of 256 of the large tiles takes as long as 0.4 + 0.62 turns of 512 middle ones, of whose last turn only a part is paid
+    // (4096 x 2048 -> 4352, 272 large tiles, 103 : 91; 36864 x 2048 -> 320 101 : 75; 12000 x 3000 -> 1100 83 : 118).
+    if (big >= 192 && K >= 2048 && (mpc_cdiv(big, 256) * 512 - 205) * 8 <= 5 * middle) return {PLAN_BIG, 1};
     if (middle >= 176) return {PLAN_MIDDLE, 1};
     const int64_t small = mpc_cdiv(M, 64) * mpc_cdiv(N, 64), k_tiles = mpc_cdiv(K, KT);
     // A k-tile takes 0.25 us with a workgroup per CU, 0.4 with two; joining the splits takes 8 us and more.  (1537 x 1000 x 1024:
