@@ -856,17 +856,19 @@ Plan plan_for(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {     // 
     const int64_t big = mpc_cdiv(M, BIG) * mpc_cdiv(N, BIG), middle = mpc_cdiv(M, 128) * mpc_cdiv(N, 128);
     // The large tile needs most CUs busy and some k-tiles to pay for its prologue and epilogue (128 x 128 tiles against it, bf16
     // with bias and gelu: 3584 x 4096 x 4096 137 us : 105; 2048 x 4096 x 4096 77 : 99; 4096 x 4096 x 1024 46 : 47; 8192 x 8192 x
-    // 512 114 : 119).  64 x 64 tiles take over where 128 x 128 ones are fewer than the CUs (768 x 4096 x 4096 44 : 39; 512 x 4096 x
-    // 4096 32 : 39).
+    // 512 114 : 119).
     // A turn of 256 of the large tiles takes as long as 0.4 + 0.62 turns of 512 middle ones, of whose last turn only a part is paid
     // (4096 x 2048 -> 4352, 272 large tiles, 103 : 91; 36864 x 2048 -> 320 101 : 75; 12000 x 3000 -> 1100 83 : 118).
     if (big >= 192 && K >= 2048 && (mpc_cdiv(big, 256) * 512 - 205) * 8 <= 5 * middle) return {PLAN_BIG, 1};
-    if (middle >= 176) return {PLAN_MIDDLE, 1};
+    // 64 x 64 tiles as long as two workgroups a CU take them all (bf16, 64 x 64 : 128 x 128: 512 x 2048 -> 4096, 512 small tiles,
+    // 18.6 : 22.2; 860 x 2993 -> 2902, 644, 51 : 37; 30000 x 1024 -> 64, 469, 14.0 : 14.4; 60000 x 256 -> 64, 938, 12.0 : 10.5).
     const int64_t small = mpc_cdiv(M, 64) * mpc_cdiv(N, 64), k_tiles = mpc_cdiv(K, KT);
-    // A k-tile takes 0.25 us with a workgroup per CU, 0.4 with two; joining the splits takes 8 us and more.  (1537 x 1000 x 1024:
-    // 10.7 us in one, 20 in two; 64 x 8192 x 8192: 44 in one, 28 in four.)
+    if (small > 512) return {PLAN_MIDDLE, 1};
+    // Split K while that gives CUs without work some, and 16 k-tiles a part: joining the parts takes 5 us and more.  (bf16, in one :
+    // as here : up to two workgroups a CU: 1000 x 2048 -> 1000, 256 tiles, 13.6 : 13.6 : 18.7; 500 x 8192 -> 500 40 : 19 : 22; 64 x
+    // 8192 -> 8192 40 : 29 : 29; 64 x 4096 -> 4096 22 : 13 : 13, with 32 k-tiles a part 16, with 8 15.)
     int splits = 1;
-    while (splits < 16 && small * splits * 2 <= 512 && k_tiles / (splits * 2) >= 16) splits *= 2;
+    while (splits < 16 && small * splits * 2 <= 256 && k_tiles / (splits * 2) >= 16) splits *= 2;
     return {PLAN_SMALL, splits};
 }
 
