@@ -10,7 +10,7 @@
 // What bounds the four kernels, and what they take (plan_for chooses; a large copy reaches 5.17 TB/s here, a large library product
 // 1574 TFLOP/s in bf16 and 2559 in e4m3): few rows, the weights' bytes: 1 x 4096 -> 4096 bf16 7.8 us, 4.3 TB/s.  64 x 64 tiles, the
 // way of a k-tile through one workgroup per CU: 1537 x 1111 -> 1000 bf16 18 us, rows at odd addresses.  128 x 128 tiles, load,
-// products and epilogue of a tile one after the other, two workgroups per CU: 36864 x 256 -> 1024 f16 with gelu 45 us, 36864 x
+// products and epilogue of a tile one after the other, two workgroups per CU: 36864 x 256 -> 1024 f16 with gelu 44 us, 36864 x
 // 1024 -> 256 e4m3 with residual 25 us.  256 x 256 tiles, L2's rate: 8192 x 4096 -> 8192 with residual and activation, bf16
 // 465 us, 1180 TFLOP/s; e4m3 309 us, 1780 TFLOP/s.
 #include "row_ops.h"
@@ -877,7 +877,8 @@ int launch_small(mpc_ctx *ctx, const LinearArgs &a, int splits, bool prepare = f
     return launch_tiles<TYPE, 64, 64, 32, 32, 4, 3>(ctx, a, splits, prepare);
 }
 // 8 waves of 64 x 32, two workgroups a CU: the second's products run beside the first's epilogue.  (36864 x 256 -> 1024 with
-// gelu: 50 us; 4 waves of 64 x 64, with one or two tiles ahead: 53; 128 x 64 tiles: 52; 256 x 128: 63.)
+// gelu, before its gelu and its last two tiles' fetches were cut: 50 us; 4 waves of 64 x 64, with one or two tiles ahead: 53; 128 x 64
+// tiles: 52; 256 x 128: 63.)
 template <int TYPE>
 int launch_middle(mpc_ctx *ctx, const LinearArgs &a, bool prepare = false) {
     return launch_tiles<TYPE, 128, 128, 64, 32, 1, 4>(ctx, a, 1, prepare);
