@@ -225,6 +225,36 @@ def test_linear_large(dtype, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
+@pytest.mark.parametrize("M,N", [(1, 40), (12, 5000), (16, 4096), (17, 4100), (30, 300), (32, 4096)])
+@pytest.mark.parametrize("K", [15, 16, 17, 129, 130, 131, 1111, 4097])
+def test_few_rows_that_begin_anywhere(dtype, M, N, K):
+    """Rows at words and between them, of any length, in front of NaN and behind it: small whole operands, exactly."""
+    from compression_amd import ops
+    g = torch.Generator().manual_seed(M * K + N)
+    for lo, width in ((0, K), (1, K + 2), (2, K + 3), (3, K + 4)):
+        x, w = torch.full((M, width), float("nan")), torch.full((N, width), float("nan"))
+        x[:, lo:lo + K] = torch.randint(-8, 9, (M, K), generator=g).float()
+        w[:, lo:lo + K] = torch.randint(-8, 9, (N, K), generator=g).float()
+        x, w = x.to(DEV), w.to(DEV)
+        one = [torch.ones(n, device=DEV) if dtype == E4M3 else None for n in (M, N)]
+        got = ops.linear(x.to(dtype)[:, lo:lo + K], w.to(dtype)[:, lo:lo + K], x_scale=one[0], weight_scale=one[1], out_dtype=F32)
+        assert torch.equal(got.double(), x[:, lo:lo + K].double() @ w[:, lo:lo + K].double().t().contiguous()), (lo, width)
+
+
+def test_prior_balance_refuses_a_workspace_between_doubles():
+    from compression_amd import _lib
+    s = torch.zeros(10, 100, device=DEV)
+    ctx = _lib.context_at(0)
+    need = ctx.lib.mpc_prior_balance_workspace_bytes(10, 100)
+    work, out = torch.zeros(need + 16, dtype=torch.uint8, device=DEV), torch.zeros(102, dtype=torch.int32, device=DEV)
+    for off, size in ((4, need), (0, need - 4)):
+        with pytest.raises(_lib.MpcError, match="workspace|misaligned"):
+            ctx.call("mpc_prior_balance", s.data_ptr(), _lib.MPC_TYPE_F32, 10, 100, 100, 1, 1.0, 1, None, work.data_ptr() + off, size, out.data_ptr(),
+                     out.data_ptr() + 4, out.data_ptr() + 404)
+    assert not bool(work.any()) and not bool(out.any())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("K", [2048, 2049, 2055, 2063, 2064, 2175, 2176, 2177, 4225])
 def test_large_tiles_whose_rows_end_anywhere(dtype, K):
     """256 x 256 tiles over rows of any length and at any address: small whole operands as above, NaN behind every row, in
