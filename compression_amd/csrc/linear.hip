@@ -850,16 +850,16 @@ struct Plan {
     int kind, splits;
 };
 
-Plan plan_for(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {     // the last three in bytes
+Plan plan_for(bool eight, int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {     // the last three in bytes
     // (rows so far apart that a tile's do not fit a buffer: the kernel that addresses each by itself)
     if (M <= 32 || BIG * xs + K > TILE_BYTES || BIG * ws + K > TILE_BYTES) return {PLAN_ROWS, 1};
     const int64_t big = mpc_cdiv(M, BIG) * mpc_cdiv(N, BIG), middle = mpc_cdiv(M, 128) * mpc_cdiv(N, 128);
     // The large tile needs most CUs busy and some k-tiles to pay for its prologue and epilogue (128 x 128 tiles against it, bf16
-    // with bias and gelu: 3584 x 4096 x 4096 137 us : 105; 2048 x 4096 x 4096 77 : 99; 4096 x 4096 x 1024 46 : 47; 8192 x 8192 x
-    // 512 114 : 119).
+    // with bias and gelu: 3584 x 4096 x 4096 137 us : 105; 2048 x 4096 x 4096 77 : 99; without: 27696 x 880 -> 5504 367 : 310; 8192 x
+    // 768 -> 8192 119 : 113; 8192 x 512 -> 8192 98 : 106; e4m3: 5000 x 1800 -> 3000 46 : 44; 10871 x 1500 -> 7431 261 : 307).
     // A turn of 256 of the large tiles takes as long as 0.4 + 0.62 turns of 512 middle ones, of whose last turn only a part is paid
     // (4096 x 2048 -> 4352, 272 large tiles, 103 : 91; 36864 x 2048 -> 320 101 : 75; 12000 x 3000 -> 1100 83 : 118).
-    if (big >= 192 && K >= 2048 && (mpc_cdiv(big, 256) * 512 - 205) * 8 <= 5 * middle) return {PLAN_BIG, 1};
+    if (big >= 192 && K >= (eight ? 2048 : 1536) && (mpc_cdiv(big, 256) * 512 - 205) * 8 <= 5 * middle) return {PLAN_BIG, 1};
     // 64 x 64 tiles as long as two workgroups a CU take them all (bf16, 64 x 64 : 128 x 128: 512 x 2048 -> 4096, 512 small tiles,
     // 18.6 : 22.2; 860 x 2993 -> 2902, 644, 51 : 37; 30000 x 1024 -> 64, 469, 14.0 : 14.4; 60000 x 256 -> 64, 938, 12.0 : 10.5).
     const int64_t small = mpc_cdiv(M, 64) * mpc_cdiv(N, 64), k_tiles = mpc_cdiv(K, KT);
@@ -886,7 +886,7 @@ int launch_middle(mpc_ctx *ctx, const LinearArgs &a, bool prepare = false) {
 
 template <int TYPE>
 int launch(mpc_ctx *ctx, const LinearArgs &a) {
-    const Plan plan = plan_for(a.M, a.N, a.K, a.xs, a.ws);
+    const Plan plan = plan_for(TYPE == MPC_TYPE_E4M3, a.M, a.N, a.K, a.xs, a.ws);
     if (plan.kind == PLAN_ROWS) {
         if (between_words(a)) return a.M <= 16 ? launch_rows<TYPE, 1, true>(ctx, a) : launch_rows<TYPE, 2, true>(ctx, a);
         return a.M <= 16 ? launch_rows<TYPE, 1, false>(ctx, a) : launch_rows<TYPE, 2, false>(ctx, a);
@@ -926,7 +926,7 @@ int mpc_linear_init(mpc_ctx *ctx) {
 extern "C" size_t mpc_linear_workspace_bytes(const mpc_linear_desc *desc) {
     if (!desc || !linear_desc_ok(*desc) || desc->M == 0) return 0;
     const int ib = mpc_type_bytes(desc->in_type);
-    const Plan plan = plan_for(desc->M, desc->N, desc->K * ib, desc->x_stride * ib, desc->w_stride * ib);
+    const Plan plan = plan_for(desc->in_type == MPC_TYPE_E4M3, desc->M, desc->N, desc->K * ib, desc->x_stride * ib, desc->w_stride * ib);
     return plan.splits > 1 ? (size_t)plan.splits * desc->M * desc->N * sizeof(float) : 0;
 }
 
