@@ -85,6 +85,22 @@ __device__ __forceinline__ void take_row(const Vec (&rows)[ROWS][P], int m, Vec 
     }
 }
 
+// Eight 16-bit values to an address between words: the words in the middle as such, a value at each end.  (36864 x 256 -> 1023
+// f16: 57 us with one access at such an address, 49 with these.  The residual's loads gain nothing from the like, and the 256 x 256
+// tiles less than they lose in registers.)
+template <typename T, typename Vec>
+__device__ __forceinline__ void store_between_words(T *to, Vec t) {
+    if constexpr (sizeof(T) == 2) {
+        typedef unsigned u32x3 __attribute__((ext_vector_type(3)));
+        typedef u32x3 u32x3_word __attribute__((aligned(4)));
+        const u32x4 v = __builtin_bit_cast(u32x4, t);
+        to[0] = t[0];
+        *(u32x3_word *)(to + 1) = u32x3{__builtin_amdgcn_alignbyte(v[1], v[0], 2), __builtin_amdgcn_alignbyte(v[2], v[1], 2),
+                                        __builtin_amdgcn_alignbyte(v[3], v[2], 2)};
+        to[7] = t[7];
+    }
+}
+
 // The rows of a lane: row0 + 16 m; its V columns are V / 8 runs of 8, n + 32 t .. n + 32 t + 7: the four lanes of a row then
 // write 64 consecutive bytes at a time.  take(m, v) gives the sums.  One rolled loop (the sums have fixed
 // registers, so take is a switch over copies): unrolled it would be tens of KB of code.
@@ -100,6 +116,7 @@ __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, i
         b[i] = a.bias && col(i) < a.N ? a.bias[col(i)] : 0.0f;
         s[i] = a.sw && col(i) < a.N ? a.sw[col(i)] : 1.0f;
     }
+    const bool between = ((uintptr_t)a.out | a.os) & 3;                     // rows of the output may begin between words
     // the residual's rows: up to four at once for 16-bit types, the next one while a row is worked on for fp32
     constexpr int KEPT = sizeof(T) == 2 ? (MF < 4 ? MF : 4) : 1;
     vec_t ahead[KEPT][P];
@@ -151,7 +168,9 @@ __device__ __forceinline__ void finish_rows(const LinearArgs &a, int64_t row0, i
 #pragma unroll
             for (int q = 0; q < PER; ++q) t[q] = (T)v[i * PER + q];
             if (col(i / RUN * 8 + 7) < a.N) {
-                *(vec_any *)(o + col(i * PER)) = t;
+                T *to = o + col(i * PER);
+                if (sizeof(T) == 2 && V < 32 && between && (uintptr_t)to & 2) store_between_words(to, t);
+                else *(vec_any *)to = t;
             } else {
 #pragma unroll
                 for (int q = 0; q < PER; ++q)
