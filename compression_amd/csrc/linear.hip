@@ -10,9 +10,9 @@
 // What bounds the four kernels, and what they take (plan_for chooses; a large copy reaches 5.17 TB/s here, a large library product
 // 1574 TFLOP/s in bf16 and 2559 in e4m3): few rows, the weights' bytes: 1 x 4096 -> 4096 bf16 7.8 us, 4.3 TB/s.  64 x 64 tiles, the
 // way of a k-tile through one workgroup per CU: 1537 x 1111 -> 1000 bf16 18 us, rows at odd addresses.  128 x 128 tiles, load,
-// products and epilogue of a tile one after the other, two workgroups per CU: 36864 x 256 -> 1024 f16 with gelu 44 us, 36864 x
-// 1024 -> 256 e4m3 with residual 25 us.  256 x 256 tiles, L2's rate: 8192 x 4096 -> 8192 with residual and activation, bf16
-// 465 us, 1180 TFLOP/s; e4m3 309 us, 1780 TFLOP/s.
+// products and epilogue of a tile one after the other, two workgroups per CU: 36864 x 256 -> 1024 f16 with gelu 42.5 us, 36864 x
+// 1024 -> 256 e4m3 with residual 24 us.  256 x 256 tiles, L2's rate: 8192 x 4096 -> 8192 with residual and activation, bf16
+// 460 to 480 us, 1200 TFLOP/s; e4m3 292 to 309 us, 1880 TFLOP/s.
 #include "row_ops.h"
 
 #include <type_traits>
