@@ -73,6 +73,23 @@ def test_rms_norm(dtype, quantize, rows, C):
         check_norm(x, r, w, 1e-6, quantize, got)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,C", [(70000, 64), (70001, 33), (33001, 192), (8300, 1024), (8200, 2047), (2100, 4096), (1100, 8191), (140000, 20),
+                                    (262144, 24), (8200, 1111), (4100, 3000), (600, 20000)])
+def test_rms_norm_of_many_rows(dtype, rows, C):
+    """Enough rows for every number of vectors a thread takes, in groups of one thread to 1024; dense, and rows between
+    words with NaN on both sides."""
+    from compression_amd import ops
+    g = torch.Generator(device=DEV).manual_seed(rows + C)
+    wide = torch.full((rows, C + 5), float("nan"), dtype=dtype, device=DEV)
+    wide[:, 1:1 + C] = torch.randn(rows, C, device=DEV, generator=g).to(dtype) * 3
+    x, r, w = wide[:, 1:1 + C], torch.randn(rows, C, device=DEV, generator=g).to(dtype), 1 + 0.3 * torch.randn(C, device=DEV, generator=g)
+    check_norm(x, r, w, 1e-6, True, ops.rms_norm(x, w, 1e-6, r, True))
+    check_norm(x, None, w, 1e-6, False, ops.rms_norm(x, w))
+    check_norm(r, None, None, 1e-6, True, ops.rms_norm(r, quantize=True))
+    check_norm(r, x, w, 1e-6, False, ops.rms_norm(r, w, residual=x))
+
+
 def test_rms_norm_strides_alignment_and_shapes():
     from compression_amd import ops
     for dtype in (F32, F16, BF16):
