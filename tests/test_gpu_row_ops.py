@@ -471,6 +471,19 @@ def test_prior_balance(dtype, T, E):
             check_balance(s, 1.0, k, mask, g, None if mask is None else mask.to(DEV))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,E", [(40000, 1), (40001, 5), (50000, 13), (40000, 30), (70001, 64), (40000, 100), (30000, 200), (20000, 300), (17001, 600),
+                                 (17000, 1024)])
+def test_prior_balance_of_many_rows(dtype, T, E):
+    """Enough rows for every width of a row's group in the blocks that go through rows in turn, and for joins over all blocks."""
+    g = torch.Generator(device=DEV).manual_seed(T + E)
+    for by_expert, k in ((False, 1), (True, min(3, E)), (False, min(5, E))):
+        s = (torch.randn(T, E, device=DEV, generator=g) * 1.5 + torch.randn(E, device=DEV, generator=g)).to(dtype)
+        s = s.t().contiguous().t() if by_expert else s
+        mask = torch.rand(T, device=DEV, generator=g) < 0.8
+        check_balance(s.cpu(), -0.7 if by_expert else 1.0, k, mask.cpu(), s, mask)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("E", [4, 64, 100, 300])
 def test_prior_balance_rows_with_little_in_them(dtype, E):
@@ -552,6 +565,22 @@ def test_prior_balance_repeats_its_bits():
     for _ in range(5):
         l2, c2, n2 = ops.prior_balance(s, top_k=2)
         assert torch.equal(loss, l2) and torch.equal(counts, c2)
+
+
+def test_prior_balance_joined_by_several_workgroups_on_two_streams():
+    """Calls in flight beside each other share nothing: the same bits as one by one."""
+    from compression_amd import ops
+    sets = [rnd(70 + i, 20000 + 3000 * i, 300).to(DEV) for i in range(2)]
+    want = [ops.prior_balance(s, top_k=2) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(40):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(ops.prior_balance(sets[i % 2], top_k=2))
+    torch.cuda.synchronize()
+    for i, t in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(t, want[i % 2]))
 
 
 # ---- all of them -----------------------------------------------------------------------------------------------------------
