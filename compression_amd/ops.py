@@ -381,8 +381,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     [N]; act MPC_ACT_NONE, _RELU, _GELU (the erf form) or _SILU; residual [..., N] in the output's type.  e4m3 operands
     bring their scales, fp32: x_scale [...] (one per row) and weight_scale [N]; 16-bit ones have none.  out_dtype: fp32,
     fp16 or bf16; default the residual's type, else x's, and fp16 for e4m3 operands.  Sums and epilogue in fp32, one
-    rounding at the end (products of e4m3 operands to about 1.5e-5 of a sum: the matrix unit's own rounding).  Values only:
-    no autograd graph."""
+    rounding at the end (above 32 rows, products of e4m3 operands to about 1.5e-5 of a sum: the matrix unit's own rounding).
+    Values only: no autograd graph."""
     index = _gpu_of(x, weight, bias, residual, x_scale, weight_scale)
     t = _OPERAND_TYPES.get(x.dtype)
     if t is None or weight.dtype != x.dtype:

@@ -258,6 +258,26 @@ def test_few_rows_that_begin_anywhere(dtype, M, N, K):
         assert torch.equal(got.double(), x[:, lo:lo + K].double() @ w[:, lo:lo + K].double().t().contiguous()), (lo, width)
 
 
+@pytest.mark.parametrize("M,N", [(1, 40), (7, 4096), (16, 100), (17, 300), (32, 5000)])
+@pytest.mark.parametrize("K", [8, 16, 100, 129, 4096])
+def test_few_rows_of_8_bit_operands_lose_nothing(M, N, K):
+    """A product of 2^14 beside ones down to 2^-8 and a scale of its own, a power of two, for every row and column: all sums
+    are multiples of 2^-8 below 2^15, exact in fp32 in any order, and what the 8-bit matrix instructions would cut off shows."""
+    from compression_amd import ops
+    g = torch.Generator().manual_seed(M + N + K)
+    sx, sw = 2.0 ** (torch.arange(M) % 5 - 2), 2.0 ** (torch.arange(N) % 7 - 3)
+    for at in sorted({0, K // 2, K - 1}):
+        x, w = (torch.randint(1, 16, (n, K), generator=g) * (torch.randint(0, 2, (n, K), generator=g) * 2 - 1) / 16.0 for n in (M, N))
+        x[:, at] = w[:, at] = 128.0
+        for lo in (0, 1):                                                 # rows at words and between them
+            gx, gw = torch.zeros(M, K + 4 * lo), torch.zeros(N, K + 4 * lo)
+            gx[:, lo:lo + K], gw[:, lo:lo + K] = x, w
+            got = ops.linear(gx.to(DEV).to(E4M3)[:, lo:lo + K], gw.to(DEV).to(E4M3)[:, lo:lo + K], x_scale=sx.to(DEV), weight_scale=sw.to(DEV),
+                             out_dtype=F32)
+            want = (x.double() @ w.double().t().contiguous()) * sx.double()[:, None] * sw.double()
+            assert torch.equal(got.cpu().double(), want), (at, lo)
+
+
 def test_prior_balance_refuses_a_workspace_between_doubles():
     from compression_amd import _lib
     s = torch.zeros(10, 100, device=DEV)
