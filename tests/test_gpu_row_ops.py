@@ -356,6 +356,45 @@ def test_linear_infinite_and_largest_sums(act, M, N):
     assert torch.equal(torch.where(got[fin].abs() < 1e-30, 0.0, got[fin]), want[fin, None].expand(-1, N))
 
 
+# sizes that reach every kernel, for tests of what follows the products: few rows, 64 x 64 tiles, K split and joined, 128 x 128, 256 x 256
+EVERY_KERNEL = [(4, 3000, 32), (40, 3000, 32), (64, 1000, 8192), (2000, 2500, 32), (3600, 3600, 2048)]
+
+
+def activation_of(v, act, odt, M, K, dtype):
+    """ops.linear's activation of the fp32 values v, through sums of 0 and a bias; every row has to be the same."""
+    from compression_amd import ops
+    N = v.numel()
+    x, w = torch.zeros(M, K, device=DEV).to(dtype), torch.zeros(N, K, device=DEV).to(dtype)
+    sx, sw = (torch.ones(M, device=DEV), torch.ones(N, device=DEV)) if dtype == E4M3 else (None, None)
+    got = ops.linear(x, w, v.to(DEV), act, None, sx, sw, odt)
+    assert torch.equal(got, got[:1].expand(M, N))
+    return got[0]
+
+
+def points(N, reach):
+    """N fp32 values: evenly spread over both signs, and of every magnitude."""
+    a = torch.linspace(-reach, reach, N - 200)
+    return torch.cat([a, *(sign * 10.0 ** torch.linspace(-30, 1, 100) for sign in (1.0, -1.0))]).float()
+
+
+@pytest.mark.parametrize("odt", [F32, F16, BF16])
+@pytest.mark.parametrize("dtype", [F16, E4M3])
+@pytest.mark.parametrize("M,N,K", EVERY_KERNEL)
+def test_gelu_to_the_output_s_rounding(M, N, K, dtype, odt):
+    """All of gelu's left tail, relative to its values there.  F(-m) = exp(-m^2 / 2) t q(t): t q(t) is good to 2^-21.5 (3.4e-7), t to
+    1.5 units of fp32 that count up to 2.4 times (4.3e-7), exp to one (1.2e-7), two products to half of one each: below 2^-19.5
+    together.  A 16-bit output's exponent m^2 / (2 ln 2) carries 2.22 half steps of itself: 1.11 m^2 2^-24 of F.  What exp leaves
+    below fp32's normal range is lost, less than 2^-127 of the result."""
+    v = points(N, 13.5)
+    got = activation_of(v, 5, odt, M, K, dtype)
+    v = v.double()
+    tail = v.abs() * 0.5 * torch.special.erfc(v.abs() / math.sqrt(2.0))
+    want = v.clamp(min=0) - tail
+    rel = 2.0 ** -19.5 + (0 if odt == F32 else 1.11 * v * v * 2.0 ** -24)
+    off = tail * rel + want.abs() * 2.0 ** -24 + 2.0 ** -127
+    within(got, want, off * (1 + u(odt)) + (0 if odt == F32 else want.abs() * u(odt)) + TINY[odt])
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("M,K", [(1, 100), (6, 1111), (50, 260), (300, 72)])
 def test_linear_special_values_stay_where_they_are(dtype, M, K):
