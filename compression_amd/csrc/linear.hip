@@ -82,8 +82,23 @@ __device__ __forceinline__ void activate(float (&v)[V], int act) {
             v[i] = fmaf(-fabsf(__builtin_fminf(v[i], 1e30f)), q * t * e, __builtin_fmaxf(v[i], 0.0f));
         }
     } else if (act == MPC_ACT_SILU) {
+        // v / (1 + exp(-v)).  exp's argument is off by 1.22 half steps, 1.22 |v| 2^-24 of the left tail: 2^-17 where silu leaves bf16's
+        // range.  An fp32 output, for which that is many units, takes the steps' losses along, by e = exp(-|v|) so that nothing
+        // overflows (36864 x 256 -> 1024 f16 -> fp32 49 us : 54).  Below exp's normal range it counts as 0, here 2^-119 and less.
+        constexpr float L = 1.44269504f, L_REST = 1.9259630e-8f;                 // 1 / ln 2
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v[i] * -1.44269504f));
+        for (int i = 0; i < V; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                float m = fabsf(v[i]);
+                m = m > 200.0f ? 200.0f : m;                                     // (a NaN stays)
+                const float z = m * -L, rest = fmaf(m, -L_REST, fmaf(m, -L, -z));
+                float e = __builtin_amdgcn_exp2f(z);
+                e = fmaf(e * rest, 0.69314718f, e);
+                v[i] = (v[i] > 0.0f ? v[i] : v[i] * e) * __builtin_amdgcn_rcpf(1.0f + e);
+            } else {
+                v[i] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v[i] * -L));
+            }
+        }
     }
 }
 

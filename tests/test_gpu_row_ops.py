@@ -395,6 +395,20 @@ def test_gelu_to_the_output_s_rounding(M, N, K, dtype, odt):
     within(got, want, off * (1 + u(odt)) + (0 if odt == F32 else want.abs() * u(odt)) + TINY[odt])
 
 
+@pytest.mark.parametrize("odt", [F32, F16, BF16])
+@pytest.mark.parametrize("M,N,K", EVERY_KERNEL)
+def test_silu_to_the_output_s_rounding(M, N, K, odt):
+    """As for gelu: exp, the sum and its reciprocal and the products are good to 2^-20.5 together; a 16-bit output's exponent carries
+    1.22 half steps of itself.  What exp leaves below fp32's normal range is lost: 90 times 2^-126 of the result."""
+    v = points(N, 100.0)
+    got = activation_of(v, 6, odt, M, K, F16)
+    v = v.double()
+    want = v / (1 + torch.exp(-v))
+    rel = 2.0 ** -20.5 + (0 if odt == F32 else 1.22 * v.clamp(max=0).abs() * 2.0 ** -24)
+    off = want.abs() * rel + 2.0 ** -119
+    within(got, want, off * (1 + u(odt)) + (0 if odt == F32 else want.abs() * u(odt)) + TINY[odt])
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, E4M3])
 @pytest.mark.parametrize("M,K", [(1, 100), (6, 1111), (50, 260), (300, 72)])
 def test_linear_special_values_stay_where_they_are(dtype, M, K):
