@@ -9,6 +9,7 @@ import atexit
 import ctypes
 import os
 import subprocess
+import threading
 import weakref
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
@@ -177,9 +178,11 @@ def ptr(t):
 
 
 class Context:
-    """One mpc_ctx per (device, HIP stream)."""
+    """One mpc_ctx on one GPU.  Without `follow_torch` it works on the stream that it was given; with it, on torch's current
+    stream of the calling thread, looked up at every call.  The C side of a context is not thread-safe: calls of several
+    threads take turns, each from the look at the stream to its error text."""
 
-    def __init__(self, device_index: int = 0, stream_handle: int = 0):
+    def __init__(self, device_index: int = 0, stream_handle: int = 0, follow_torch: bool = False):
         self.lib = load()
         h = c_void_p()
         rc = self.lib.mpc_create(device_index, c_void_p(stream_handle), ctypes.byref(h))
@@ -188,11 +191,23 @@ class Context:
         self.handle = h
         self.device_index = device_index
         self.stream_handle = stream_handle
+        self.lock = threading.RLock()         # (re-entered where collecting garbage frees a layer in the middle of a call)
+        self.torch_stream = None
+        if follow_torch:
+            import torch
+            self.torch_stream = torch._C._cuda_getCurrentRawStream       # (torch.cuda.current_stream(i).cuda_stream, without the object)
         register_owner(self)
 
     def set_stream(self, stream_handle: int):
-        self.check(self.lib.mpc_set_stream(self.handle, c_void_p(stream_handle)))
-        self.stream_handle = stream_handle
+        """For a context of one's own; the shared ones go by torch's current stream."""
+        if self.torch_stream is not None:
+            raise MpcError("this context works on torch's current stream (torch.cuda.stream(...)); for another make a Context of your own")
+        self._use_stream(stream_handle)
+
+    def _use_stream(self, stream_handle: int):
+        with self.lock:
+            self.check(self.lib.mpc_set_stream(self.handle, c_void_p(stream_handle)))
+            self.stream_handle = stream_handle
 
     def check(self, rc: int):
         if rc != 0:
@@ -200,9 +215,16 @@ class Context:
             raise MpcError(f"libmpc error {rc}: {msg.decode() if msg else ''}")
 
     def call(self, name: str, *args):
-        rc = getattr(self.lib, name)(self.handle, *args)
-        if rc != 0:
-            self.check(rc)
+        if name == "mpc_set_stream":          # (stream_handle says what the C side has)
+            return self.set_stream(*(getattr(a, "value", a) for a in args))
+        with self.lock:
+            if self.torch_stream is not None:
+                stream = self.torch_stream(self.device_index)
+                if stream != self.stream_handle:
+                    self._use_stream(stream)
+            rc = getattr(self.lib, name)(self.handle, *args)
+            if rc != 0:
+                self.check(rc)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -217,10 +239,11 @@ class Context:
 
 
 _contexts = {}
+_contexts_lock = threading.Lock()
 
 
 def context_for(device) -> Context:
-    """Context bound to `device` (a torch.device) and to torch's current stream on it."""
+    """The context of `device` (a torch.device), shared by all threads; its `call` works on torch's current stream there."""
     import torch
 
     if device.type != "cuda":
@@ -230,12 +253,10 @@ def context_for(device) -> Context:
 
 def context_at(index: int) -> Context:
     """context_for, by the GPU's index."""
-    import torch
-
     ctx = _contexts.get(index)
     if ctx is None:
-        ctx = _contexts[index] = Context(index, 0)
-    stream = torch._C._cuda_getCurrentRawStream(index)     # (what torch.cuda.current_stream(index).cuda_stream is, without the object)
-    if stream != ctx.stream_handle:
-        ctx.set_stream(stream)
+        with _contexts_lock:
+            ctx = _contexts.get(index)
+            if ctx is None:
+                ctx = _contexts[index] = Context(index, 0, follow_torch=True)
     return ctx

@@ -917,7 +917,7 @@ class ConvLayer:
         self._rgb16 = f16 and self.small_cout and cout <= 4 and cin % 64 == 0 and cin <= 256
         ctx = context_for(w.device)
         h = c_void_p()
-        ctx.check(ctx.lib.mpc_conv_create(ctx.handle, ctypes.byref(self.desc), ptr(w), ptr(b), ptr(be), ptr(ga), ctypes.byref(h)))
+        ctx.call("mpc_conv_create", ctypes.byref(self.desc), ptr(w), ptr(b), ptr(be), ptr(ga), ctypes.byref(h))
         self.handle = h
         self._lib = ctx.lib
         _lib.register_owner(self)

@@ -764,6 +764,33 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
 
 
+def test_threads_on_streams_of_their_own():
+    """Four threads, each with its stream and its tensors, at once: every result is the one that the thread's call has alone."""
+    import threading
+    from compression_amd import _lib, ops
+    sets = [head_tensors(80 + 10 * i, r) for i, r in enumerate((300, 5, 1536, 40))]
+    want = [head(ops, _lib, t) for t in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(40):
+                    got = head(ops, _lib, sets[i])
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        bad.append(i)
+        except BaseException as e:                        # noqa: BLE001 (reported below)
+            bad.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+
+
 @pytest.mark.parametrize("M,N,K,dtype", [(3, 500, 700, BF16), (40, 200, 9000, F16), (300, 300, 200, E4M3), (3000, 1500, 256, F16),
                                          (3600, 3600, 1024, BF16), (3600, 3600, 2048, E4M3)])
 def test_every_kernel_of_linear_in_a_graph_and_on_two_streams(M, N, K, dtype):

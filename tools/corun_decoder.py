@@ -40,8 +40,7 @@ def run(beside):
             with torch.cuda.stream(sa):
                 sa.wait_event(go)
                 if occupier:                                # (a -DMPC_EXPERIMENT_OCCUPIER build: a sleeping kernel of the decoder's footprint)
-                    ctx = _lib.context_for(dev)
-                    ctx.check(ctx.lib.mpc_experiment_occupier(ctx.handle, 660, 18484, 370, ctypes.c_void_p(sink.data_ptr())))
+                    _lib.context_for(dev).call("mpc_experiment_occupier", 660, 18484, 370, ctypes.c_void_p(sink.data_ptr()))
                 else:
                     job = m.decode_batch_begin(strings, idx, h, w)
         with torch.cuda.stream(sb):
