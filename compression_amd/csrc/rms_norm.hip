@@ -22,6 +22,11 @@ struct NormArgs {
     int group;                                     // threads of a row, a power of two
 };
 
+// (mean square + eps)^(-1/2); 0 where that is 0 (eps = 0 and a row of zeros), so that the row stays one of zeros
+__device__ __forceinline__ float row_inverse(float sum, int channels, float eps) {
+    const float d = sum / (float)channels + eps;
+    return d == 0.0f ? 0.0f : 1.0f / sqrtf(d);
+}
 
 // s = top / 448 for the row's largest |v| (by its bits: the order of non-negative floats, with NaN above infinity)
 __device__ __forceinline__ float row_scale(unsigned top) {
@@ -108,7 +113,7 @@ __global__ __launch_bounds__(NORM_MAX_THREADS) void rms_norm_kernel(NormArgs a) 
         sum = 0.0f;
         for (int i = 0; i < G / 64; ++i) sum += part[tid / G * (G / 64) + i];
     }
-    const float inv = 1.0f / sqrtf(sum / (float)C + a.eps);
+    const float inv = row_inverse(sum, C, a.eps);
 
     unsigned top = 0;
 #pragma unroll
@@ -208,7 +213,7 @@ __global__ __launch_bounds__(NORM_MAX_THREADS) void rms_norm_long_kernel(NormArg
     __syncthreads();
     sum = 0.0f;
     for (int i = 0; i < NT / 64; ++i) sum += part[i];
-    const float inv = 1.0f / sqrtf(sum / (float)C + a.eps);
+    const float inv = row_inverse(sum, C, a.eps);
     auto value = [&](int c) { return at(c) * inv * (a.weight ? a.weight[c] : 1.0f); };
     if (!eight) {
         for (int64_t c = tid; c < C; c += NT) ((T *)a.y)[row * C + c] = (T)value(c);

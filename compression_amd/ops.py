@@ -337,8 +337,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     x, residual: [..., C] fp32, fp16 or bf16, rows evenly spaced (a slice of wider rows is fine), residual of x's shape and
     type; weight fp32 [C] or None.  -> v in x's type, or with quantize (q, scale): e4m3 values [..., C] and fp32 [...],
     v ~ q * scale, what `linear` takes as x and x_scale.  With a residual h (x's type, rounded once; the norm is taken of
-    the unrounded sum) is returned behind them: (v, h) or (q, scale, h).  Rows of zeros have scale 1.  Values only, like the
-    rest of the library: no autograd graph."""
+    the unrounded sum) is returned behind them: (v, h) or (q, scale, h).  Rows of zeros give zeros, with scale 1, for eps = 0
+    too.  Values only, like the rest of the library: no autograd graph."""
     index = _gpu_of(x, weight, residual)
     dtype = x.dtype
     t = _ROW_TYPES.get(dtype)

@@ -349,7 +349,9 @@ enum { MPC_TYPE_F32 = 0, MPC_TYPE_F16 = 1, MPC_TYPE_BF16 = 2, MPC_TYPE_E4M3 = 3 
  * (the norm is taken of the unrounded sum), y: v, both dense [rows][channels].  y_type == type: v rounded once, scale
  * must be NULL.  y_type == MPC_TYPE_E4M3: scale[i] = max_c |v| / 448, at least 2^-126, 1 for a row of zeros, and
  * y = e4m3(v / scale[i]), nearest, ties to even.  A NaN anywhere in a row makes all of that row's y (and scale) NaN, an
- * infinity makes its scale NaN.  Sums are in fp32: rows whose squares add up beyond 3e38 give zeros.
+ * infinity makes its scale NaN.  Sums are in fp32: rows whose squares add up beyond 3e38 give zeros.  eps may be 0: a row
+ * of zeros then gives zeros, as does one whose squares vanish in fp32 (values below 2^-75), and a mean square below 2^-126
+ * has fewer bits.
  * Outputs overlap no input and no other output.  rows may be 0. */
 int mpc_rms_norm(mpc_ctx *ctx, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
                  const float *weight, int64_t rows, int64_t channels, float eps, int type, void *h, void *y, int y_type,

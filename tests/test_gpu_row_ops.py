@@ -129,6 +129,29 @@ def test_rms_norm_special_values(C):
     assert math.isnan(float(y[5, C - 1])) and not bool(y[5, :C - 1].any()) and math.isnan(float(s[5]))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("C", [5, 192, 1111, 4096, 20000, 70000])
+def test_rms_norm_without_eps(dtype, C):
+    """eps = 0: rows of zeros stay zeros with scale 1 and so do rows whose squares vanish in fp32, NaN stays in its row, other
+    rows are normalised."""
+    from compression_amd import ops
+    x = rnd(C, 8, C).to(dtype)
+    x[1], x[3], x[6] = 0.0, -0.0, (1e-30 if dtype != F16 else 0.0)
+    x[5, C // 2] = float("nan")
+    x[7] = (x[7].float() * 2.0 ** -14).to(dtype)
+    w, ok, zero = 1 + 0.1 * rnd(C + 1, C), [0, 2, 4, 7], [1, 3, 6]
+    r = torch.zeros_like(x)
+    for res in (None, r):
+        y = ops.rms_norm(x.to(DEV), w.to(DEV), 0.0, None if res is None else r.to(DEV))
+        q = ops.rms_norm(x.to(DEV), w.to(DEV), 0.0, None if res is None else r.to(DEV), quantize=True)
+        y = y if res is None else y[0]
+        q, s = q[0].float().cpu(), q[1].cpu()
+        check_norm(x[ok], None, w, 0.0, False, y.cpu()[ok])
+        check_norm(x[ok], None, w, 0.0, True, (q[ok].to(E4M3), s[ok]))
+        assert not bool(y.cpu()[zero].any()) and not bool(q[zero].any()) and bool((s[zero] == 1).all())
+        assert bool(torch.isnan(y[5]).all()) and bool(torch.isnan(q[5]).all()) and math.isnan(float(s[5]))
+
+
 def test_rms_norm_writes_its_rows_only():
     """Through the C ABI: guards around every output stay as they were."""
     from compression_amd import _lib
