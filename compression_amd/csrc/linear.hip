@@ -576,21 +576,42 @@ int allow_lds(mpc_ctx *ctx, const void *kernel, size_t bytes) {
     return MPC_OK;
 }
 
+// The tiles, of bm x bn outputs and a workgroup each, in as many launches as they take: one has fewer than 2^32 threads.
+template <typename F>
+void in_parts(const LinearArgs &a, int bm, int bn, int threads, F run) {
+    const int64_t most = MPC_LAUNCH_THREADS / threads, all_n = mpc_cdiv(a.N, bn), tiles_n = all_n < most ? all_n : most;
+    const int64_t rows = most / tiles_n * bm, columns = tiles_n * bn;
+    const int ob = mpc_type_bytes(a.out_type);
+    for (int64_t m = 0; m < a.M; m += rows) {
+        for (int64_t n = 0; n < a.N; n += columns) {
+            LinearArgs part = a;
+            part.M = a.M - m < rows ? a.M - m : rows;
+            part.N = a.N - n < columns ? a.N - n : columns;
+            part.tiles_m = (int)mpc_cdiv(part.M, bm);
+            part.tiles_n = (int)mpc_cdiv(part.N, bn);
+            part.x = a.x + m * a.xs;
+            part.w = a.w + n * a.ws;
+            if (a.sx) part.sx = a.sx + m, part.sw = a.sw + n;
+            if (a.bias) part.bias = a.bias + n;
+            if (a.res) part.res = a.res + m * a.rs + n * ob;
+            part.out = a.out + m * a.os + n * ob;
+            run(part);
+        }
+    }
+}
+
 template <int TYPE, int BM, int BN, int WM, int WN, int DEPTH, int PER_SIMD>
-int launch_tiles(mpc_ctx *ctx, LinearArgs a, int splits, bool prepare = false) {
+int launch_tiles(mpc_ctx *ctx, const LinearArgs &a, int splits, bool prepare = false) {
     constexpr size_t lds = 2 * (BM + BN) * KT;
     auto kern = linear_tile_kernel<TYPE, BM, BN, WM, WN, DEPTH, PER_SIMD>;
     if (prepare) return allow_lds(ctx, (const void *)kern, lds);
-    const int64_t tm = mpc_cdiv(a.M, BM), tn = mpc_cdiv(a.N, BN);
-    MPC_REQUIRE(ctx, tm * tn < (1ll << 30), "linear: too many tiles");
-    a.tiles_m = (int)tm;
-    a.tiles_n = (int)tn;
-    kern<<<dim3((unsigned)(tm * tn), (unsigned)splits), dim3(64 * (BM / WM) * (BN / WN)), lds, ctx->stream>>>(a);
+    constexpr int NT = 64 * (BM / WM) * (BN / WN);
+    in_parts(a, BM, BN, NT, [&](const LinearArgs &part) {
+        kern<<<dim3((unsigned)(part.tiles_m * part.tiles_n), (unsigned)splits), dim3(NT), lds, ctx->stream>>>(part);
+    });
     MPC_CHECK_LAUNCH(ctx, "linear_tile");
-    if (splits > 1) {
-        const int64_t blocks = mpc_cdiv(a.M * ((a.N + 3) / 4), 256);
-        MPC_REQUIRE(ctx, blocks < (1ll << 31), "linear: too many outputs to join");
-        linear_join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, ctx->stream>>>(a, splits);
+    if (splits > 1) {                                             // (few tiles: one part)
+        linear_join_kernel<<<dim3((unsigned)mpc_cdiv(a.M * ((a.N + 3) / 4), 256)), dim3(256), 0, ctx->stream>>>(a, splits);
         MPC_CHECK_LAUNCH(ctx, "linear_join");
     }
     return MPC_OK;
@@ -768,13 +789,13 @@ __global__ __launch_bounds__(256, 1) void linear_big_kernel(LinearArgs a) {
 }
 
 template <int TYPE>
-int launch_big(mpc_ctx *ctx, LinearArgs a, bool prepare = false) {
+int launch_big(mpc_ctx *ctx, const LinearArgs &a, bool prepare = false) {
     constexpr size_t lds = 2 * 2 * BIG * KT;
     auto kern = linear_big_kernel<TYPE>;
     if (prepare) return allow_lds(ctx, (const void *)kern, lds);
-    a.tiles_m = (int)mpc_cdiv(a.M, BIG);
-    a.tiles_n = (int)mpc_cdiv(a.N, BIG);
-    kern<<<dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(256), lds, ctx->stream>>>(a);
+    in_parts(a, BIG, BIG, 256, [&](const LinearArgs &part) {
+        kern<<<dim3((unsigned)(part.tiles_m * part.tiles_n)), dim3(256), lds, ctx->stream>>>(part);
+    });
     MPC_CHECK_LAUNCH(ctx, "linear_big");
     return MPC_OK;
 }
@@ -903,13 +924,13 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(LinearArgs a) {
 bool between_words(const LinearArgs &a) { return ((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.xs | (uintptr_t)a.ws) % 4 != 0; }
 
 template <int TYPE, int MF, bool ODD>
-int launch_rows(mpc_ctx *ctx, LinearArgs a) {
-    const int64_t tiles_n = mpc_cdiv(a.N, 16), blocks = tiles_n * mpc_cdiv(a.M, 16 * MF);
-    MPC_REQUIRE(ctx, blocks < (1ll << 31), "linear: too many tiles");
-    a.tiles_n = (int)tiles_n;
-    // up to a workgroup per CU: 16 waves, so that the CU's whole share of w is on its way; more: 8 waves, two workgroups a CU
-    if (blocks <= 256) linear_rows_kernel<TYPE, MF, 16, ODD><<<dim3((unsigned)blocks), dim3(1024), 0, ctx->stream>>>(a);
-    else linear_rows_kernel<TYPE, MF, 8, ODD><<<dim3((unsigned)blocks), dim3(512), 0, ctx->stream>>>(a);
+int launch_rows(mpc_ctx *ctx, const LinearArgs &a) {
+    in_parts(a, 16 * MF, 16, 1024, [&](const LinearArgs &part) {
+        const int blocks = part.tiles_m * part.tiles_n;
+        // up to a workgroup per CU: 16 waves, so that the CU's whole share of w is on its way; more: 8 waves, two workgroups a CU
+        if (blocks <= 256) linear_rows_kernel<TYPE, MF, 16, ODD><<<dim3((unsigned)blocks), dim3(1024), 0, ctx->stream>>>(part);
+        else linear_rows_kernel<TYPE, MF, 8, ODD><<<dim3((unsigned)blocks), dim3(512), 0, ctx->stream>>>(part);
+    });
     MPC_CHECK_LAUNCH(ctx, "linear_rows");
     return MPC_OK;
 }

@@ -234,6 +234,22 @@ __global__ __launch_bounds__(NORM_MAX_THREADS) void rms_norm_long_kernel(NormArg
     for (int64_t c = tid; c < C; c += NT) ((uint8_t *)a.y)[row * C + c] = (uint8_t)(e4m3_pack2<false>(value(c) * back, 0.0f, 0) & 0xff);
 }
 
+// The rows in as many launches as they take: one has fewer than 2^32 threads (`per_row` for each row).
+template <typename T, bool Q, typename F>
+void in_parts(const NormArgs &a, int per_row, F run) {
+    const int64_t most = MPC_LAUNCH_THREADS / per_row;
+    for (int64_t first = 0; first < a.rows; first += most) {
+        NormArgs part = a;
+        part.rows = a.rows - first < most ? a.rows - first : most;
+        part.x = (const T *)a.x + first * a.xs;
+        if (a.res) part.res = (const T *)a.res + first * a.rs;
+        if (a.h) part.h = (T *)a.h + first * a.channels;
+        part.y = (char *)a.y + first * a.channels * (Q ? 1 : sizeof(T));
+        if (Q) part.scale = a.scale + first;
+        run(part);
+    }
+}
+
 // Vectors per thread and threads per row.  More vectors mean more loads in flight and no barrier (a row within a wave), as
 // long as the card stays full of waves, a row's threads reach over 64 bytes, 512 with more than two vectors, and no more slots
 // stay empty; fewer empty slots come first.  (bf16 + residual -> 8 bit, in us, one vector a thread : this rule: 50000 x 2048 138 : 137,
@@ -244,7 +260,9 @@ int launch(mpc_ctx *ctx, NormArgs a) {
     constexpr int W = 16 / sizeof(T);
     const int64_t vectors = mpc_cdiv(a.channels, W);
     if (vectors > (int64_t)NORM_MOST * NORM_MAX_THREADS) {
-        rms_norm_long_kernel<T><<<dim3((unsigned)a.rows), dim3(NORM_MAX_THREADS), 0, ctx->stream>>>(a, Q);
+        in_parts<T, Q>(a, NORM_MAX_THREADS, [&](const NormArgs &part) {
+            rms_norm_long_kernel<T><<<dim3((unsigned)part.rows), dim3(NORM_MAX_THREADS), 0, ctx->stream>>>(part, Q);
+        });
         MPC_CHECK_LAUNCH(ctx, "rms_norm_long");
         return MPC_OK;
     }
@@ -261,14 +279,16 @@ int launch(mpc_ctx *ctx, NormArgs a) {
     }
     a.group = group;
     const int threads = group > 256 ? group : 256;
-    const dim3 grid((unsigned)mpc_cdiv(a.rows, threads / group)), block(threads);
-    switch (vpt) {
-        case 1: rms_norm_kernel<T, 1, Q><<<grid, block, 0, ctx->stream>>>(a); break;
-        case 2: rms_norm_kernel<T, 2, Q><<<grid, block, 0, ctx->stream>>>(a); break;
-        case 3: rms_norm_kernel<T, 3, Q><<<grid, block, 0, ctx->stream>>>(a); break;
-        case 4: rms_norm_kernel<T, 4, Q><<<grid, block, 0, ctx->stream>>>(a); break;
-        default: rms_norm_kernel<T, NORM_MOST, Q><<<grid, block, 0, ctx->stream>>>(a);
-    }
+    in_parts<T, Q>(a, group, [&](const NormArgs &part) {
+        const dim3 grid((unsigned)mpc_cdiv(part.rows, threads / group)), block(threads);
+        switch (vpt) {
+            case 1: rms_norm_kernel<T, 1, Q><<<grid, block, 0, ctx->stream>>>(part); break;
+            case 2: rms_norm_kernel<T, 2, Q><<<grid, block, 0, ctx->stream>>>(part); break;
+            case 3: rms_norm_kernel<T, 3, Q><<<grid, block, 0, ctx->stream>>>(part); break;
+            case 4: rms_norm_kernel<T, 4, Q><<<grid, block, 0, ctx->stream>>>(part); break;
+            default: rms_norm_kernel<T, NORM_MOST, Q><<<grid, block, 0, ctx->stream>>>(part);
+        }
+    });
     MPC_CHECK_LAUNCH(ctx, "rms_norm");
     return MPC_OK;
 }

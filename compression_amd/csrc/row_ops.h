@@ -9,6 +9,10 @@ inline int mpc_type_bytes(int type) {
     return type == MPC_TYPE_F32 ? 4 : type == MPC_TYPE_F16 || type == MPC_TYPE_BF16 ? 2 : type == MPC_TYPE_E4M3 ? 1 : 0;
 }
 
+// Most threads of a launch: HIP takes fewer than 2^32, and where there are more it runs what their number leaves modulo 2^32,
+// without an error.
+constexpr int64_t MPC_LAUNCH_THREADS = 1ll << 31;
+
 #if defined(__HIPCC__)
 constexpr float E4M3_MAX = 448.0f;
 

@@ -699,6 +699,39 @@ def test_offsets_beyond_32_bits():
     check_balance(s.cpu(), 1.0, 1, None, s, None)
 
 
+def test_more_threads_than_a_launch_takes():
+    """HIP launches fewer than 2^32 threads: more rows or columns than that go in several launches.  The operands are one row
+    over and over, what is added to the product differs from place to place."""
+    from compression_amd import ops
+    N, K = (1 << 27) + 77, 8                                              # few rows: 512 threads for 16 columns
+    for dtype in (F16, E4M3):
+        x, w = (torch.arange(1, 9.0, device=DEV) / 4).to(dtype)[None], torch.ones(1, K, device=DEV).to(dtype)
+        sx, sw = (torch.full((1,), 2.0, device=DEV), torch.arange(N, device=DEV, dtype=torch.int32) % 3 + 1.0) if dtype == E4M3 else (None, None)
+        bias = (torch.arange(N, device=DEV, dtype=torch.int32) % 251).float()
+        res = (torch.arange(N, device=DEV, dtype=torch.int32) % 127).to(F16)[None]
+        got = ops.linear(x, w.expand(N, K), bias, 3, res, sx, sw, F16)
+        want = (9.0 * (1 if sw is None else 2 * sw) + bias + res[0].float()).to(F16)
+        assert torch.equal(got[0], want)
+        del bias, res, got, want, sw
+    M = (1 << 30) + 133                                                   # 128 x 128 tiles: 512 threads for 128 rows
+    res = (torch.arange(M, device=DEV, dtype=torch.int32) % 127).to(F16)[:, None]
+    got = ops.linear(torch.ones(1, K, dtype=F16, device=DEV).expand(M, K), torch.ones(1, K, dtype=F16, device=DEV), residual=res)
+    assert torch.equal(got, res + 8)
+    M = (1 << 28) + 45                                                    # rows of w too far apart for tiles: 512 threads for 32 rows
+    far = torch.as_strided(torch.ones((1 << 22) + K, dtype=F16, device=DEV), (2, K), (1 << 22, 1))
+    res = (torch.arange(2 * M, device=DEV, dtype=torch.int32) % 127).to(F16).view(M, 2)
+    got = ops.linear(torch.ones(1, K, dtype=F16, device=DEV).expand(M, K), far, residual=res)
+    assert torch.equal(got, res + 8)
+    del res, got
+    rows, C = (1 << 30) + 5, 13                                           # a norm's four threads a row
+    x = rnd(90, 1, C).to(DEV)
+    q1, s1 = ops.rms_norm(x, quantize=True)
+    q, s = ops.rms_norm(x.expand(rows, C), quantize=True)
+    assert bool((s == s1).all())
+    for i in range(0, rows, 1 << 27):
+        assert bool((q[i:i + (1 << 27)].view(torch.uint8) == q1.view(torch.uint8)).all()), i
+
+
 def head(ops, _lib, t):
     """Scores for the priors from a latent, the way a learned choice would make them: norm, product, product back onto the
     residual stream, scores, balance and its gradient."""
