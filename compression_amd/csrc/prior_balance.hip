@@ -580,7 +580,8 @@ int check(mpc_ctx *ctx, const void *scores, int type, int64_t rows, int experts,
     MPC_REQUIRE(ctx, top_k > 0 && top_k <= experts, "prior_balance: top_k = %d of %d experts", top_k, experts);
     MPC_REQUIRE(ctx, rows >= 0 && rows < (1ll << 31) / top_k, "prior_balance: %lld rows", (long long)rows);
     MPC_REQUIRE(ctx, rs >= 0 && es >= 0, "prior_balance: negative stride");
-    MPC_REQUIRE(ctx, scale != 0.0f && scale > -INFINITY && scale < INFINITY, "prior_balance: scale = %g", (double)scale);
+    // (2^127 and more would leave fp32 with exp2's factor)
+    MPC_REQUIRE(ctx, scale != 0.0f && fabsf(scale) < 0x1p127f, "prior_balance: scale = %g", (double)scale);
     MPC_REQUIRE(ctx, rows == 0 || (scores && (uintptr_t)scores % mpc_type_bytes(type) == 0), "prior_balance: null or misaligned pointer");
     return MPC_OK;
 }

@@ -380,7 +380,8 @@ int mpc_linear_forward(mpc_ctx *ctx, const mpc_linear_desc *desc, const void *x,
 
 /* How evenly the experts (the priors of a competition) are used, as a loss, with its gradient.  scores [rows][experts] of
  * `type` (F32, F16, BF16) at element row * row_stride + expert * expert_stride (either layout of the competition's
- * totals); z = scale * scores (scale finite, not 0; negative for costs), p = softmax(z) of a row.  A row counts if
+ * totals); z = scale * scores (scale not 0, |scale| < 2^127; negative for costs), p = softmax(z) of a row, 0 for a
+ * score more than 3.4e38 from the row's best.  A row counts if
  * mask[row] != 0 (mask uint8, may be NULL) and it holds a z above -infinity (or a NaN).  It chooses its top_k largest z
  * above -infinity, among equal ones those of the lowest index; a NaN is never chosen.  With R the rows that count,
  *   counts[e] = rows that chose e,  f = counts / (top_k R),  P[e] = mean over those rows of p,

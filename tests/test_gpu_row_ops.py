@@ -606,6 +606,20 @@ def test_prior_balance_rows_with_little_in_them(dtype, E):
                 check_balance(s, scale, k, mask, g.t().contiguous().t(), mask.to(torch.uint8).to(DEV))
 
 
+def test_prior_balance_scales_at_the_ends_of_fp32():
+    """The largest and smallest scales give what the definition does; beyond 2^127 they are refused."""
+    from compression_amd import _lib, ops
+    s = rnd(3, 50, 64)
+    for scale, size in ((2.0 ** 126.9, 2.0 ** -127), (-(2.0 ** 126.9), 2.0 ** -125), (2.0 ** -126, 2.0 ** 125), (2.0 ** 126, 1.0)):
+        t = s * size
+        check_balance(t, scale, 2, None, t.to(DEV), None)
+    for scale in (2.0 ** 127, -3.4e38, -math.inf):
+        with pytest.raises(_lib.MpcError, match="scale"):
+            ops.prior_balance(s.to(DEV), scale)
+        with pytest.raises(_lib.MpcError, match="scale"):
+            ops.prior_balance_grad(s.to(DEV), torch.zeros(64, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV), scale=scale)
+
+
 def test_prior_balance_nan_and_no_rows():
     from compression_amd import ops
     s = rnd(1, 10, 64)
