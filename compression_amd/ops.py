@@ -434,6 +434,8 @@ def _balance_args(scores, scale, top_k, mask):
     if t is None or scores.dim() != 2:
         raise MpcError(f"prior_balance: scores must be [rows, experts] float32, float16 or bfloat16 (got {scores.dtype} {tuple(scores.shape)})")
     T, E = scores.shape
+    if not 0 < top_k <= E < 1 << 31:                     # (ctypes would take them modulo 2^32)
+        raise MpcError(f"prior_balance: top_k = {top_k} of {E} experts")
     if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (T,) or not mask.is_contiguous()):
         raise MpcError(f"prior_balance: mask must be {T} contiguous bool values, got {mask.dtype} {tuple(mask.shape)}")
     return (scores.data_ptr(), t, T, E, *scores.stride(), scale, top_k, _addr(mask))

@@ -42,6 +42,16 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_balance_takes_no_number_modulo_its_type():
+    scores = torch.zeros(2, 8)
+    assert ops._balance_args(scores, 1.0, 8, None)[7] == 8
+    for top_k in (0, -1, 9, (1 << 32) + 1, 1 - (1 << 32)):
+        with pytest.raises(MpcError, match="top_k"):
+            ops._balance_args(scores, 1.0, top_k, None)
+    with pytest.raises(MpcError, match="experts"):
+        ops._balance_args(torch.zeros(1, 1).expand(2, (1 << 32) + 4), 1.0, 1, None)
+
+
 def test_linear_workspace_of_a_bad_description_is_zero():
     lib = _lib.load()
     d = _lib.LinearDesc(_lib.MPC_TYPE_F32, _lib.MPC_TYPE_F32, 0, 4, 4, 4, 4, 4, 0, 4)
