@@ -31,9 +31,22 @@ extern "C" {
 
 const char *mpc_version(void) { return "libmpc 0.3 gfx950 (hand-written HIP: f32 / split-fp16 / fp16 MFMA transforms with LDS-patch kernels, prior competition, MRS1 rANS)"; }
 
+namespace {
+// While one lives, this thread may make calls that a stream capture forbids by default (here: loading the library's code, looking
+// up its symbols; none of them touches the captured stream), so that a process's first call may be a captured one.
+struct capture_relaxed {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    bool on = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+    ~capture_relaxed() {
+        if (on) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    }
+};
+}  // namespace
+
 int mpc_create(int device_id, void *stream, mpc_ctx **out) {
     if (!out) return MPC_EINVAL;
     *out = nullptr;
+    const capture_relaxed relaxed;
     int n = 0;
     if (hipGetDeviceCount(&n) != hipSuccess || device_id < 0 || device_id >= n) return MPC_EHIP;
     mpc_device_guard guard(device_id);          // the caller's current device is put back on return

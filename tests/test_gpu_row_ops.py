@@ -893,6 +893,32 @@ def test_every_kernel_of_linear_in_a_graph_and_on_two_streams(M, N, K, dtype):
         assert torch.equal(y, want[i % 2])
 
 
+def test_a_process_s_first_call_may_be_a_captured_one():
+    """In a process of its own: nothing of the library has run when the capture begins."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from compression_amd import ops
+x, w = torch.randn(8, 256, device="cuda:0").bfloat16(), torch.randn(64, 256, device="cuda:0").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ops.linear(ops.rms_norm(x), w)
+    loss, _, _ = ops.prior_balance(y)
+for i in range(3):
+    x.mul_(1.5)
+    graph.replay()
+    want = ops.linear(ops.rms_norm(x), w)
+    assert torch.equal(y, want) and torch.equal(loss, ops.prior_balance(want)[0])
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True,
+                          timeout=100)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
 def test_balance_in_a_graph_by_itself():
     """Captured forward and gradient, replayed on changed scores with other calls of the same operators between."""
     from compression_amd import ops
