@@ -43,6 +43,22 @@ struct LinearArgs {
 };
 
 // ---- epilogue ---------------------------------------------------------------------------------------------------------
+// log2 F(-m), F the normal distribution, as a polynomial in m (constant first) for gelu in 16-bit outputs: fitted as far as gelu's
+// left tail stays in the type, and falling beyond.  With its roundings F is good to 2^-15.3 of itself for fp16 (m up to 5.8), 2^-12.1 for
+// bf16 (13.3), a twentieth and a ninth of half a step, and to 3.5e-7 in absolute terms.
+template <typename T>
+struct TailExponent;
+template <>
+struct TailExponent<f16_t> {
+    static constexpr float P[] = {-0.999999583f, -1.15112638f, -0.459036678f, -0.0529954731f, 0.0077384538f, -0.000608425296f, -1.10764704e-05f,
+                                  6.52565996e-06f, -3.8450608e-07f};
+};
+template <>
+struct TailExponent<bf16_t> {
+    static constexpr float P[] = {-0.999999046f, -1.15114987f, -0.458879262f, -0.0533608608f, 0.00811367016f, -0.000794931198f, 3.39617181e-05f,
+                                  1.83778775e-06f, -3.23463979e-07f, 1.63099578e-08f, -2.98272906e-10f};
+};
+
 // V consecutive outputs of row m from column n on, T their type.  v: the sums.
 template <typename T, int V>
 __device__ __forceinline__ void activate(float (&v)[V], int act) {
@@ -50,36 +66,44 @@ __device__ __forceinline__ void activate(float (&v)[V], int act) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];            // (a NaN stays)
     } else if (act == MPC_ACT_GELU) {
-        // gelu(v) = max(v, 0) - |v| F(-|v|), F the normal distribution: F(-m) = exp(-m^2 / 2) t q(t), t = 1 / (1 + 0.33 m), q of
-        // degree 8 fitted for the least largest error relative to F on 0 <= m <= 13.5 (a linear program over 2000 points), beyond
-        // which exp is 0.  t q(t) is good to 2^-21.5 with its roundings.  The exponent is off by three half steps, 1.1 m^2 2^-24 of
-        // F: 2^-16 where gelu leaves bf16's range, 2^-19 where it leaves fp16's.  An fp32 output takes what those steps lose along
-        // and is good to 2^-20.  gelu(inf) = inf (1e30 * 0 is subtracted); at -inf the formula's -inf * 0 is NaN, here as in
-        // silu.  (A fifth-degree polynomial of log2 F, good to 3e-7 of |v| but to no digit of F at v = -8, takes half as many
-        // instructions: 36864 x 256 -> 1024 50 us : 55 in f16, 45 : 50 in bf16; 8192 x 4096 -> 8192 e4m3 with residual 303 : 318.)
-        constexpr float C = 0.72134752f, C_REST = 9.6298152e-9f;                    // 1 / (2 ln 2)
+        // gelu(v) = max(v, 0) - |v| F(-|v|), F the normal distribution.  gelu(inf) = inf (1e30 * 0 is subtracted); at -inf the
+        // formula's -inf * 0 is NaN, here as in silu.  All fits are for the least largest error, by linear programs.
+        if constexpr (sizeof(T) == 2) {
+            // F(-m) = 2^P(m), one exponential and as few other instructions as the type's half step allows (TailExponent).  (36864 x 256
+            // -> 1024, this : a formula good to 2^-16 for both, with a reciprocal : degree 5, good to 3e-7 of |v| but to no digit at v = -8:
+            // f16 53 us : 55 : 50, bf16 48 : 50 : 44; 8192 x 4096 -> 8192 e4m3 with residual 308 : 318 : 300.)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float m = fabsf(v[i]), e;
-            if constexpr (sizeof(T) == 4) {
+            for (int i = 0; i < V; ++i) {
+                const float m = fabsf(v[i]);
+                constexpr int N = sizeof(TailExponent<T>::P) / sizeof(float);
+                float q = TailExponent<T>::P[N - 1];
+#pragma unroll
+                for (int k = N - 2; k >= 0; --k) q = fmaf(m, q, TailExponent<T>::P[k]);
+                v[i] = fmaf(-fabsf(__builtin_fminf(v[i], 1e30f)), __builtin_amdgcn_exp2f(q), __builtin_fmaxf(v[i], 0.0f));
+            }
+        } else {
+            // F(-m) = exp(-m^2 / 2) t q(t), t = 1 / (1 + 0.33 m), q of degree 8 fitted relative to F on 0 <= m <= 13.5, beyond which exp is
+            // 0: t q(t) is good to 2^-21.5 with its roundings, and what those of the exponent lose is taken along: 2^-20 in all.
+            constexpr float C = 0.72134752f, C_REST = 9.6298152e-9f;             // 1 / (2 ln 2)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float m = fabsf(v[i]);
                 m = m > 20.0f ? 20.0f : m;                                       // (a NaN stays)
                 const float m2 = m * m, z = m2 * -C;
                 const float rest = fmaf(fmaf(m, m, -m2), -C, fmaf(m2, -C_REST, fmaf(m2, -C, -z)));
-                e = __builtin_amdgcn_exp2f(z);
+                float e = __builtin_amdgcn_exp2f(z);
                 e = fmaf(e * rest, 0.69314718f, e);
-            } else {
-                e = __builtin_amdgcn_exp2f(m * m * -C);
+                const float t = __builtin_amdgcn_rcpf(fmaf(m, 0.33f, 1.0f));
+                float q = fmaf(t, -0.0211830456f, 0.124867819f);
+                q = fmaf(t, q, -0.270793527f);
+                q = fmaf(t, q, 0.228645995f);
+                q = fmaf(t, q, -0.0592148937f);
+                q = fmaf(t, q, 0.122923814f);
+                q = fmaf(t, q, 0.110794663f);
+                q = fmaf(t, q, 0.13233906f);
+                q = fmaf(t, q, 0.131620139f);
+                v[i] = fmaf(-fabsf(__builtin_fminf(v[i], 1e30f)), q * t * e, __builtin_fmaxf(v[i], 0.0f));
             }
-            const float t = __builtin_amdgcn_rcpf(fmaf(m, 0.33f, 1.0f));
-            float q = fmaf(t, -0.0211830456f, 0.124867819f);
-            q = fmaf(t, q, -0.270793527f);
-            q = fmaf(t, q, 0.228645995f);
-            q = fmaf(t, q, -0.0592148937f);
-            q = fmaf(t, q, 0.122923814f);
-            q = fmaf(t, q, 0.110794663f);
-            q = fmaf(t, q, 0.13233906f);
-            q = fmaf(t, q, 0.131620139f);
-            v[i] = fmaf(-fabsf(__builtin_fminf(v[i], 1e30f)), q * t * e, __builtin_fmaxf(v[i], 0.0f));
         }
     } else if (act == MPC_ACT_SILU) {
         // v / (1 + exp(-v)).  exp's argument is off by 1.22 half steps, 1.22 |v| 2^-24 of the left tail: 2^-17 where silu leaves bf16's

@@ -362,8 +362,8 @@ int mpc_rms_norm(mpc_ctx *ctx, const void *x, int64_t x_stride, const void *resi
  * x [M][K] and w [N][K] of in_type (F16, BF16 or E4M3), residual (may be NULL) and out [M][N] of out_type (F32, F16 or
  * BF16); rows at multiples of the strides (in elements, below 2^40), values of a row consecutive.  bias (may be NULL) fp32 [N].
  * x_scale fp32 [M] and w_scale fp32 [N]: with E4M3 operands, both; with 16-bit ones, NULL.  act: MPC_ACT_NONE, _RELU,
- * _GELU or _SILU (both NaN at -infinity: -inf * 0; the left tails are good to 2^-20 of their values for an F32 out, to
- * 2^-16 for a 16-bit one, and may be 0 below 2^-119).  Sums and the epilogue are in fp32, out is rounded once; above 32 rows
+ * _GELU or _SILU (both NaN at -infinity: -inf * 0; the left tails are good to 2^-20 of their values for an F32 out, 2^-15
+ * for an F16 and 2^-12 for a BF16 one, and may be 0 below 2^-119).  Sums and the epilogue are in fp32, out is rounded once; above 32 rows
  * the products of E4M3 operands carry the 8-bit matrix instructions' own rounding (2^-13 of the largest of eight neighbouring
  * products, see linear.hip), up to 32 rows they are exact in fp32.  out may be the residual itself (same
  * address and stride); otherwise it overlaps no input.  M may be 0.  A work split over K goes through `workspace`

@@ -404,17 +404,20 @@ def points(N, reach):
 @pytest.mark.parametrize("dtype", [F16, E4M3])
 @pytest.mark.parametrize("M,N,K", EVERY_KERNEL)
 def test_gelu_to_the_output_s_rounding(M, N, K, dtype, odt):
-    """All of gelu's left tail, relative to its values there.  F(-m) = exp(-m^2 / 2) t q(t): t q(t) is good to 2^-21.5 (3.4e-7), t to
-    1.5 units of fp32 that count up to 2.4 times (4.3e-7), exp to one (1.2e-7), two products to half of one each: below 2^-19.5
-    together.  A 16-bit output's exponent m^2 / (2 ln 2) carries 2.22 half steps of itself: 1.11 m^2 2^-24 of F.  What exp leaves
-    below fp32's normal range is lost, less than 2^-127 of the result."""
+    """All of gelu's left tail, relative to its values there.  fp32: F(-m) = exp(-m^2 / 2) t q(t): t q(t) is good to 2^-21.5 (3.4e-7), t
+    to 1.5 units that count up to 2.4 times (4.3e-7), exp to one (1.2e-7), two products and a sum to half of one each, and of the exponent
+    nothing is lost: below 2^-19.5 together.  16 bits: F(-m) = 2^P(m), evaluated in fp32 on 800001 points of the fit's range (to 5.8
+    and to 13.3) good to 2^-15.33 and 2^-12.18 with P's roundings, and exp to one unit; beyond the range both F and 2^P(m) m are below
+    half of the type's smallest value.  What exp leaves below fp32's normal range is lost: in fp32 |v| times 2^-126 t q(t), with |v| <
+    13.4 and t q(t) < 0.031 there, so less than 2^-127; in 16 bits F itself below 2^-126, which it is from |v| = 12.95 on, so less than
+    12.96 * 2^-126 < 2^-122."""
     v = points(N, 13.5)
     got = activation_of(v, 5, odt, M, K, dtype)
     v = v.double()
     tail = v.abs() * 0.5 * torch.special.erfc(v.abs() / math.sqrt(2.0))
     want = v.clamp(min=0) - tail
-    rel = 2.0 ** -19.5 + (0 if odt == F32 else 1.11 * v * v * 2.0 ** -24)
-    off = tail * rel + want.abs() * 2.0 ** -24 + 2.0 ** -127
+    rel = {F32: 2.0 ** -19.5, F16: 2.0 ** -15.3, BF16: 2.0 ** -12.1}[odt]
+    off = tail * rel + want.abs() * 2.0 ** -24 + 2.0 ** (-127 if odt == F32 else -122)
     within(got, want, off * (1 + u(odt)) + (0 if odt == F32 else want.abs() * u(odt)) + TINY[odt])
 
 
