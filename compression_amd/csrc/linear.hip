@@ -8,11 +8,11 @@
 // one row, 16 bytes of a 16-bit type, and the four lanes of a row with 32 consecutive ones.
 //
 // What bounds the four kernels, and what they take (plan_for chooses; a large copy reaches 5.17 TB/s here, a large library product
-// 1574 TFLOP/s in bf16 and 2559 in e4m3): few rows, the weights' bytes: 1 x 4096 -> 4096 bf16 7.8 us, 4.3 TB/s.  64 x 64 tiles, the
-// way of a k-tile through one workgroup per CU: 1537 x 1111 -> 1000 bf16 18 us, rows at odd addresses.  128 x 128 tiles, load,
-// products and epilogue of a tile one after the other, two workgroups per CU: 36864 x 256 -> 1024 f16 with gelu 42.5 us, 36864 x
-// 1024 -> 256 e4m3 with residual 24 us.  256 x 256 tiles, L2's rate: 8192 x 4096 -> 8192 with residual and activation, bf16
-// 460 to 480 us, 1200 TFLOP/s; e4m3 292 to 309 us, 1880 TFLOP/s.
+// 1574 TFLOP/s in bf16 and 3090 in e4m3): few rows, the weights' bytes: 1 x 4096 -> 4096 bf16 7.6 us, 4.4 TB/s.  64 x 64 tiles, the
+// way of a k-tile through the one or two workgroups of a CU: 1537 x 1111 -> 1000 bf16 18.6 us, rows at odd addresses.  128 x 128 tiles,
+// load, products and epilogue of a tile one after the other, two workgroups per CU: 36864 x 256 -> 1024 f16 with gelu 44 us, 36864 x
+// 1024 -> 256 e4m3 with residual 24 us.  256 x 256 tiles, at 2.0 GHz under their load with the matrix pipes busy 56 % of the cycles:
+// 8192 x 4096 -> 8192 with residual and activation, bf16 460 us, 1200 TFLOP/s; e4m3 301 us, 1830 TFLOP/s.
 #include "row_ops.h"
 
 #include <type_traits>

@@ -8,8 +8,8 @@
 // in a fixed order and in double.  Scores whose experts are not consecutive (the competition writes its totals prior by
 // prior) go through an LDS tile, read and, for the gradient, written along the rows.
 //
-// 1M x 64 bf16, top 2, with a mask: forward 46 to 56 us, bound by its vector instructions (an exponential and two rounds of
-// the choice per score); gradient 48 to 51 us, 5.2 TB/s.  1536 x 64 fp32, expert by expert: 10 us with its join + 5.3, latency.
+// 1M x 64 bf16, top 2, with a mask: forward 47 us and its join 7, bound by its vector instructions (an exponential and two rounds
+// of the choice per score); gradient 49 us, 5.2 TB/s.  1536 x 64 fp32, expert by expert: 5.5 us, join 3.3, gradient 5.3, latency.
 #include "row_ops.h"
 
 #include <type_traits>

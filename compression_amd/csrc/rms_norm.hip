@@ -3,7 +3,7 @@
 //
 // A row is read once: its threads keep h in registers (fp32) across the sum, the largest value and the output.  The kernel
 // moves x, r, h and y once each and does about ten operations a value, so memory bounds it: 32768 x 4096 bf16 with residual
-// to 8 bit 176 us, 5.3 TB/s; without either 99 us, 5.4 TB/s; 36864 x 192 f16 6.8 us out of L2; one row 3.4 us.
+// to 8 bit 176 us, 5.3 TB/s; without either 99 us, 5.4 TB/s; 36864 x 192 f16 6.9 us out of L2; one row 3.4 us.
 #include "row_ops.h"
 
 namespace {
