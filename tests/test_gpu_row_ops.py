@@ -390,7 +390,8 @@ def activation_of(v, act, odt, M, K, dtype):
     x, w = torch.zeros(M, K, device=DEV).to(dtype), torch.zeros(N, K, device=DEV).to(dtype)
     sx, sw = (torch.ones(M, device=DEV), torch.ones(N, device=DEV)) if dtype == E4M3 else (None, None)
     got = ops.linear(x, w, v.to(DEV), act, None, sx, sw, odt)
-    assert torch.equal(got, got[:1].expand(M, N))
+    bits = got.view(torch.int32 if odt == F32 else torch.int16)           # (NaN as well)
+    assert torch.equal(bits, bits[:1].expand(M, N))
     return got[0]
 
 
@@ -419,6 +420,40 @@ def test_gelu_to_the_output_s_rounding(M, N, K, dtype, odt):
     rel = {F32: 2.0 ** -19.5, F16: 2.0 ** -15.3, BF16: 2.0 ** -12.1}[odt]
     off = tail * rel + want.abs() * 2.0 ** -24 + 2.0 ** (-127 if odt == F32 else -122)
     within(got, want, off * (1 + u(odt)) + (0 if odt == F32 else want.abs() * u(odt)) + TINY[odt])
+
+
+@pytest.mark.parametrize("odt", [F32, F16, BF16])
+@pytest.mark.parametrize("act", [0, 3, 5, 6])
+@pytest.mark.parametrize("M,N,K", EVERY_KERNEL)
+def test_activations_at_the_ends_of_fp32(M, N, K, act, odt):
+    """Infinities, NaN and the largest sums in every type of output (gelu and silu of -inf are NaN: -inf * 0)."""
+    ends = torch.tensor([math.inf, -math.inf, math.nan, 3.4e38, -3.4e38, 1e30, -1e30, 1e19, -1e19, 1e5, -1e5, 200.0, -200.0, 20.0, -20.0, 0.0, -0.0])
+    v = ends.repeat(N // len(ends) + 1)[:N]
+    got = activation_of(v, act, odt, M, K, F16).cpu()
+    want = act64(v.double(), act) if act != 6 else v.double() / (1 + torch.exp(-v.double()))
+    want = torch.where((want.abs() < 1e-30), 0.0, want)
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), nan)
+    far = ~nan & (v.abs() != 20)                          # (no activation's bend is in reach of these: their values are exact)
+    got = torch.where(got.abs() < 1e-30, torch.zeros_like(got), got)
+    assert torch.equal(got[far], want[far].float().to(odt))
+    near = v.abs() == 20
+    within(got[near], want[near], want[near].abs() * (u(odt) + 2.0 ** -19) + TINY[odt] + 1e-30)
+
+
+@pytest.mark.parametrize("M,N,K", EVERY_KERNEL + [(17, 300, 100), (300, 300, 129)])
+def test_scales_of_rows_and_columns_exactly(M, N, K):
+    """8-bit operands of small whole numbers, scales that differ from row to row and from column to column (powers of two), a whole
+    bias and residual: exact in fp32, so a scale in the wrong place shows."""
+    from compression_amd import ops
+    g = torch.Generator().manual_seed(M + N + K)
+    x, w = (torch.randint(-2, 3, (n, K), generator=g).float().to(DEV) for n in (M, N))
+    sx, sw = (2.0 ** torch.randint(-3, 3, (n,), generator=g).float().to(DEV) for n in (M, N))
+    bias, res = torch.randint(-9, 9, (N,), generator=g).float().to(DEV), torch.randint(-9, 9, (M, N), generator=g).float().to(DEV)
+    got = ops.linear(x.to(E4M3), w.to(E4M3), bias, 0, res, sx, sw, F32)
+    # (whole sums of at most 2^15 by 2^-6 to 2^4: multiples of 2^-6 below 2^10, or of more below 2^20)
+    want = (x.double() @ w.double().t().contiguous()) * sx.double()[:, None] * sw.double() + bias.double() + res.double()
+    assert torch.equal(got.double(), want)
 
 
 @pytest.mark.parametrize("odt", [F32, F16, BF16])
