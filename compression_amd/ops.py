@@ -445,7 +445,7 @@ def prior_balance(scores: torch.Tensor, scale: float = 1.0, top_k: int = 1, mask
     """How evenly the experts of a choice are used: -> (loss fp32 scalar, counts int32 [E], n_rows int32 [1]).
 
     scores [rows, E] fp32, fp16 or bf16 in any layout (the competition's totals [K, n_loc] as `totals.t()` with a negative
-    scale: costs in bits weigh -ln 2); p = softmax(scale * scores).  Every row that counts (mask true, something above
+    scale: costs in bits weigh -ln 2; |scale| < 2^127); p = softmax(scale * scores).  Every row that counts (mask true, something above
     -infinity) chooses its top_k best, ties to the lowest index.  loss = E * sum_e f_e P_e with f the share of the choices and
     P the mean of p: 1 for even use, up to E where one expert takes all; 0 without rows.  counts are the choices per
     expert.  Everything stays on the device; the order of the sums is fixed."""
